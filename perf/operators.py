@@ -117,7 +117,8 @@ def prepare(case, seed):
         if own:
             from linatt_b200.quant import W4Weight
 
-            s["w"] = W4Weight(s["packed"], s["scales"], s["zeros"], in_features=K, group_size=gs)
+            s["w"] = W4Weight(s["packed"], s["scales"], s["zeros"], in_features=K, group_size=gs,
+                              activation=None if case["act"] == "none" else case["act"])
     elif case["op"] == "step":
         B, HQ, H, D, Dv, K = (case[n] for n in ("B", "HQ", "H", "D", "Dv", "conv"))
         C = HQ * D + H * D + H * Dv
@@ -166,7 +167,7 @@ def run(s):
         if op == "w4":
             from linatt_b200.quant import w4_linear
 
-            return w4_linear(s["x"], s["w"], activation=None if s["case"]["act"] == "none" else s["case"]["act"])
+            return w4_linear(s["x"], s["w"])
         if op == "step":
             q, k, v = s["step"](s["qkv"], s["pos"], s["ring"])
             return {"q": q, "k": k, "v": v, "ring": s["ring"]}
