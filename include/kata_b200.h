@@ -555,6 +555,95 @@ KATA_API int kata_add_rmsnorm_fwd(const kata_add_rmsnorm_args* args, kata_stream
 KATA_API size_t kata_add_rmsnorm_bwd_workspace_bytes(const kata_add_rmsnorm_args* args);
 KATA_API int kata_add_rmsnorm_bwd(const kata_add_rmsnorm_args* args, kata_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Linear layer with 4-bit weights, for generation: y = x W^T with
+ *   W[n,k] = scale[n, k/group] * (code[n,k] - zero[n, k/group]),   codes 0..15, zero 8 when not given,
+ * and, for a gated weight (gate rows 0..N/2-1, up rows N/2..N-1), y = silu(gate) * up with N/2 columns.
+ * The codes and scales are exact in the products, which are summed in fp32 per group; only y is rounded.
+ * `codes`, `scales` and `zeros` are in this library's tile layout, written once by kata_w4_pack (16-byte
+ * aligned buffers of the sizes that kata_w4_layout gives).  group: 32, 64 or a multiple of 128.
+ * dtype is that of x, y and the scales (f32 too: x is then used in full, as three bf16 parts).
+ * No counterpart in the reference, whose layers keep 16- or 32-bit weights.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  const void* codes;   /* from kata_w4_pack */
+  const void* scales;  /* from kata_w4_pack, dtype */
+  const void* zeros;   /* from kata_w4_pack, or NULL: all 8 */
+  int N, K, group, dtype;
+  int gated;           /* 1: rows are [gate; up], y has N/2 columns */
+} kata_w4_weight;
+
+/* Bytes of the three laid-out buffers (each may be NULL) for a weight of these sizes; KATA_OK or an error. */
+KATA_API int kata_w4_layout(const kata_w4_weight* w, size_t* code_bytes, size_t* scale_bytes, size_t* zero_bytes);
+/* Lays out a row-major quantised weight: packed (N, 4 ceil(K/32)) int32, code k of a row in bits
+ * 4 (k % 8) .. +3 of word k / 8 (codes past K are ignored); scales (N, ceil(K/group)) dtype; zeros
+ * (N, ceil(K/group)) uint8 in 0..15, or NULL.  Writes all bytes of the three buffers. */
+KATA_API int kata_w4_pack(const void* packed, const void* scales, const void* zeros, const kata_w4_weight* w,
+                          kata_stream_t stream);
+/* y (rows, ldy) = x (rows, ldx) W^T; row strides in elements, both with contiguous columns.  x of any
+ * alignment that its type has.  status: as for kata_attn_fwd. */
+KATA_API int kata_w4_linear(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy,
+                            long long rows, int* status, kata_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * One token per sequence between the fused q/k/v projection and kata_decode_step: causal short
+ * convolution (+ SiLU) on a ring of earlier inputs, the norm of each q and k head, the rotation.
+ *   a[c] = sum_{j<K} conv_w[c,j] x_{p-K+1+j}[c],  y = silu(a)   (K = 0: y = x)
+ *   norm 0 none, 1 l2, 2 RMS (with q_weight / k_weight, NULL: no scale), and rope 0..2 as kata_rownorm_*
+ * A row of x is [HQ heads of D | H heads of D | H heads of Dv].  ring (B, K-1, C) holds input p of a
+ * sequence in slot p % (K-1) (zeros before its first token) and is updated: the slot of `positions[b]`
+ * receives this input.  Channels in fp32 between the steps; q (B,HQ,D), k (B,H,D), v (B,H,Dv) are
+ * rounded once.  A sequence whose position is negative, or beyond the T rows of cos / sin when rope != 0,
+ * gets NaN and leaves its ring alone.  D and Dv multiples of 8 up to 256; K <= 4; rope 1: R = D, rope 2:
+ * R a multiple of 16 that divides D.  x, ring, q, k and v 16-byte aligned, ldx a multiple of 16 bytes.
+ * Counterpart in the reference: none (its layer keeps no cache, kata/layer.py:421-492); for whole
+ * sequences it calls fla's ShortConvolution, norms and RotaryEmbedding (kata/layer.py:296-372).
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  const float* conv_w;    /* (C, K) fp32, C = (HQ + H) D + H Dv; NULL when K = 0 */
+  const float* q_weight;  /* (D) fp32 or NULL */
+  const float* k_weight;  /* (D) fp32 or NULL */
+  const float* cos;       /* (T, R/2) fp32 or NULL */
+  const float* sin;
+  int dtype, HQ, H, D, Dv, K;
+  int norm_q, norm_k, rope, R, T;
+  float eps_q, eps_k;
+} kata_qkv_step_args;
+
+KATA_API int kata_qkv_step(const kata_qkv_step_args* args, const void* x, long long ldx, const int64_t* positions,
+                           void* ring, void* q, void* k, void* v, long long B, kata_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The next token of each of B rows of V logits, from one uniform number a row.  With m the row's
+ * maximum and T its temperature, a token's mass is rint(exp((x - m) / T) 2^40); all sums are sums of
+ * these whole numbers, so a token depends on its row, settings and number alone.  Tokens are ordered
+ * by logit, equal logits by index.  Kept are the first top_k tokens (top_k <= 0 or >= V: all); of
+ * them those with less than top_p times their mass before them (top_p >= 1: all); and of these the
+ * ones with exp((x - m) / T) >= min_p; the first token always.  Drawn is the first token in vocabulary
+ * order whose inclusive kept mass exceeds u times the whole.  T <= 0: the first token of the order.
+ * NaN logits count as -inf, which is never drawn; a row with nothing else gives token -1 and logprob
+ * -inf.  logprob is the drawn token's log probability among the kept tokens (0 for T <= 0).
+ * Each setting is a (B) array, or NULL and then the `_all` value.  V <= 2^22.
+ * No counterpart in the reference, which does not generate.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  const void* logits;        /* (B, ld) dtype, columns [0, V) */
+  const float* u;            /* (B) in [0, 1) */
+  const float* temperature;  /* (B) or NULL */
+  const int* top_k;          /* (B) or NULL */
+  const float* top_p;        /* (B) or NULL */
+  const float* min_p;        /* (B) or NULL */
+  int64_t* token;            /* (B) [out] */
+  float* logprob;            /* (B) [out] */
+  long long ld, B;
+  int V, dtype;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+} kata_sample_args;
+
+KATA_API int kata_sample(const kata_sample_args* args, kata_stream_t stream);
+
 /* Human-readable name of a KATA_ERR_* code (static storage). */
 KATA_API const char* kata_strerror(int code);
 

@@ -130,6 +130,31 @@ class AddRmsNormArgs(ctypes.Structure):
     ]
 
 
+class W4WeightArgs(ctypes.Structure):
+    _fields_ = [
+        ("codes", c_void_p), ("scales", c_void_p), ("zeros", c_void_p),
+        ("N", c_int), ("K", c_int), ("group", c_int), ("dtype", c_int), ("gated", c_int),
+    ]
+
+
+class QkvStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("conv_w", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p), ("cos", c_void_p), ("sin", c_void_p),
+        ("dtype", c_int), ("HQ", c_int), ("H", c_int), ("D", c_int), ("Dv", c_int), ("K", c_int),
+        ("norm_q", c_int), ("norm_k", c_int), ("rope", c_int), ("R", c_int), ("T", c_int),
+        ("eps_q", c_float), ("eps_k", c_float),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("u", c_void_p), ("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p),
+        ("min_p", c_void_p), ("token", c_void_p), ("logprob", c_void_p),
+        ("ld", ctypes.c_longlong), ("B", ctypes.c_longlong), ("V", c_int), ("dtype", c_int),
+        ("temperature_all", c_float), ("top_k_all", c_int), ("top_p_all", c_float), ("min_p_all", c_float),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -227,6 +252,19 @@ def lib() -> ctypes.CDLL:
                 f.argtypes = [ctypes.POINTER(AddRmsNormArgs), c_void_p]
             L.kata_add_rmsnorm_bwd_workspace_bytes.restype = c_size_t
             L.kata_add_rmsnorm_bwd_workspace_bytes.argtypes = [ctypes.POINTER(AddRmsNormArgs)]
+            P_W4 = ctypes.POINTER(W4WeightArgs)
+            P_SZ = ctypes.POINTER(c_size_t)
+            L.kata_w4_layout.restype = c_int
+            L.kata_w4_layout.argtypes = [P_W4, P_SZ, P_SZ, P_SZ]
+            L.kata_w4_pack.restype = c_int
+            L.kata_w4_pack.argtypes = [c_void_p, c_void_p, c_void_p, P_W4, c_void_p]
+            L.kata_w4_linear.restype = c_int
+            L.kata_w4_linear.argtypes = [P_W4, c_void_p, c_ll, c_void_p, c_ll, c_ll, c_void_p, c_void_p]
+            L.kata_qkv_step.restype = c_int
+            L.kata_qkv_step.argtypes = ([ctypes.POINTER(QkvStepArgs), c_void_p, c_ll] + [c_void_p] * 5 +
+                                        [c_ll, c_void_p])
+            L.kata_sample.restype = c_int
+            L.kata_sample.argtypes = [ctypes.POINTER(SampleArgs), c_void_p]
             if L.kata_abi_version() != ABI_VERSION:
                 raise RuntimeError(f"libkata_b200 ABI {L.kata_abi_version()} != expected {ABI_VERSION}")
             _lib = L
@@ -260,6 +298,23 @@ def require_cuda(*ts: torch.Tensor | None) -> torch.device:
 
 def stream_handle(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+class _Stay:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_STAY = _Stay()
+
+
+def on_device(dev: torch.device):
+    """``torch.cuda.device(dev)``, or nothing to enter where ``dev`` is current already (a launch of a
+    few microseconds would wait for the two device switches)."""
+    return _STAY if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 # Per-device status word that bounded device-side waits write on timeout.

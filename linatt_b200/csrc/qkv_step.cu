@@ -1,0 +1,252 @@
+// qkv_step.cu -- one token's way from the fused q/k/v projection to the recurrent attention step:
+//   a[c] = sum_{j<K} w[c,j] x_{p-K+1+j}[c],  y = silu(a)            causal short convolution (K <= 4)
+//   q, k heads: y / sqrt(sum y^2 + eps) or y rsqrt(mean y^2 + eps) w     norm of each head
+//   q, k heads: rotation by the position's angles                        (as kata_rownorm_*)
+// The K - 1 earlier inputs of a sequence are a ring: input p lies in slot p % (K - 1), so a step reads
+// the whole ring and overwrites only the oldest slot.
+//
+// HBM-bound: (K + 1) reads and writes of a row of inputs and one of outputs.  A thread owns eight
+// neighbouring channels; the lanes of a head are neighbours in a warp, which sums the norm and swaps
+// the halves of a rotation through shuffles.  A thread takes several sequences, so that the
+// convolution's weights are read once.  Between the steps values stay in fp32; q, k and v are rounded
+// once.
+#include <algorithm>
+
+#include "attn_common.cuh"
+#include "host_util.h"
+#include "kata_b200.h"
+
+namespace kata {
+namespace {
+
+struct StepParams {
+  const void* x;
+  const long long* pos;
+  void* ring;
+  void* q;
+  void* k;
+  void* v;
+  const float* conv_w;
+  const float* qw;
+  const float* kw;
+  const float* cos;
+  const float* sin;
+  long long ldx;
+  int B, HQ, H, D, Dv, norm_q, norm_k, rope, R, T;
+  float eps_q, eps_k;
+  int lph;   // lanes per head slot, a power of two
+  int rows;  // sequences per thread
+};
+
+constexpr int kQT = 128;
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+  } else {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    uint4 u;
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = u;
+  } else {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+template <typename T, int K>
+__global__ void __launch_bounds__(kQT) qkv_step_kernel(const StepParams p) {
+  const int slots = p.HQ + 2 * p.H;
+  const int spc = kQT / p.lph;  // head slots per CTA
+  const int slot = blockIdx.x * spc + threadIdx.x / p.lph;
+  const int e0 = (threadIdx.x % p.lph) * 8, lane = threadIdx.x & 31;
+  const int kind = slot < p.HQ ? 0 : slot < p.HQ + p.H ? 1 : 2;
+  const int dim = kind == 2 ? p.Dv : p.D;
+  const bool live = slot < slots && e0 < dim;
+  const int C = (p.HQ + p.H) * p.D + p.H * p.Dv;
+  const int head = kind == 0 ? slot : kind == 1 ? slot - p.HQ : slot - p.HQ - p.H;
+  const int c0 = (kind == 0 ? 0 : kind == 1 ? p.HQ * p.D : (p.HQ + p.H) * p.D) + head * dim + e0;
+  const int norm = kind == 0 ? p.norm_q : kind == 1 ? p.norm_k : 0;
+  const float* nw = kind == 0 ? p.qw : kind == 1 ? p.kw : nullptr;
+  const float eps = kind == 0 ? p.eps_q : p.eps_k;
+
+  float w[K ? K : 1][8];
+  if (K && live) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < K; ++j) w[j][i] = p.conv_w[static_cast<size_t>(c0 + i) * K + j];
+  }
+  for (int r = 0; r < p.rows; ++r) {
+    const int b = blockIdx.y * p.rows + r;
+    if (b >= p.B) break;  // the same for the whole CTA
+    const long long pos = p.pos[b];
+    const bool bad = pos < 0 || (p.rope && pos >= p.T);
+    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      const T* xp = static_cast<const T*>(p.x) + b * p.ldx + c0;
+      load8<T>(xp, y);
+      if constexpr (K > 0) {
+        float xin[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xin[i] = y[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= w[K - 1][i];
+        if constexpr (K > 1) {
+          T* rp = static_cast<T*>(p.ring) + static_cast<size_t>(b) * (K - 1) * C + c0;
+          const int at = bad ? 0 : static_cast<int>(pos % (K - 1));
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j) {  // input pos - (K - 1) + j is in slot (pos + j) % (K - 1)
+            int sl = at + j;
+            if (sl >= K - 1) sl -= K - 1;
+            float o[8];
+            load8<T>(rp + static_cast<size_t>(sl) * C, o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = fmaf(w[j][i], o[i], y[i]);
+          }
+          if (!bad) store8<T>(rp + static_cast<size_t>(at) * C, xin);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] / (1.f + expf(-y[i]));
+      }
+    }
+    if (p.norm_q | p.norm_k) {  // the same for the whole warp, whose heads may be of all three kinds
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+      for (int o = p.lph / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float s = rsqrtf((norm == 2 ? ss / dim : ss) + eps);
+      if (norm && live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= (norm == 2 && nw) ? s * nw[e0 + i] : s;
+      }
+    }
+    if (p.rope == 1 && kind < 2 && live) {
+      const size_t at = static_cast<size_t>(bad ? 0 : pos) * (p.R / 2) + e0 / 2;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float c = p.cos[at + i / 2], s = p.sin[at + i / 2], a0 = y[i], a1 = y[i + 1];
+        y[i] = a0 * c - a1 * s;
+        y[i + 1] = a0 * s + a1 * c;
+      }
+    } else if (p.rope == 2) {
+      const int half = p.R / 2, r0 = e0 % p.R;
+      const bool first = r0 < half;
+      float o[8];
+      const int from = first ? lane + half / 8 : lane - half / 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, y[i], from & 31);
+      if (kind < 2 && live) {
+        const size_t at = static_cast<size_t>(bad ? 0 : pos) * half + (first ? r0 : r0 - half);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float c = p.cos[at + i], s = p.sin[at + i];
+          y[i] = first ? y[i] * c - o[i] * s : y[i] * c + o[i] * s;
+        }
+      }
+    }
+    if (live) {
+      if (bad) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7fffffff);
+      }
+      T* out = kind == 0 ? static_cast<T*>(p.q) + (static_cast<size_t>(b) * p.HQ + head) * p.D
+               : kind == 1 ? static_cast<T*>(p.k) + (static_cast<size_t>(b) * p.H + head) * p.D
+                           : static_cast<T*>(p.v) + (static_cast<size_t>(b) * p.H + head) * p.Dv;
+      store8<T>(out + e0, y);
+    }
+  }
+}
+
+template <typename T>
+void launch_step(const StepParams& p, int K, cudaStream_t st) {
+  const int spc = kQT / p.lph, slots = p.HQ + 2 * p.H;
+  const dim3 grid((slots + spc - 1) / spc, (p.B + p.rows - 1) / p.rows);
+  switch (K) {
+    case 0: qkv_step_kernel<T, 0><<<grid, kQT, 0, st>>>(p); break;
+    case 1: qkv_step_kernel<T, 1><<<grid, kQT, 0, st>>>(p); break;
+    case 2: qkv_step_kernel<T, 2><<<grid, kQT, 0, st>>>(p); break;
+    case 3: qkv_step_kernel<T, 3><<<grid, kQT, 0, st>>>(p); break;
+    default: qkv_step_kernel<T, 4><<<grid, kQT, 0, st>>>(p); break;
+  }
+}
+
+}  // namespace
+}  // namespace kata
+
+using namespace kata;
+
+extern "C" int kata_qkv_step(const kata_qkv_step_args* a, const void* x, long long ldx, const int64_t* positions,
+                             void* ring, void* q, void* k, void* v, long long B, kata_stream_t stream) {
+  if (!a) return KATA_ERR_INVALID;
+  if (a->dtype != KATA_DTYPE_F32 && a->dtype != KATA_DTYPE_BF16 && a->dtype != KATA_DTYPE_F16) return KATA_ERR_DTYPE;
+  if (B < 0 || B > 0x7fffffff || a->H < 1 || a->HQ < a->H || a->HQ % a->H || a->HQ > 65536) return KATA_ERR_SHAPE;
+  if (a->D < 8 || a->D > 256 || a->D % 8 || a->Dv < 8 || a->Dv > 256 || a->Dv % 8) return KATA_ERR_SHAPE;
+  if (a->K < 0 || a->K > 4) return KATA_ERR_UNSUPPORTED;
+  if (a->norm_q < 0 || a->norm_q > 2 || a->norm_k < 0 || a->norm_k > 2 || a->rope < 0 || a->rope > 2) return KATA_ERR_INVALID;
+  if (a->rope) {
+    if (!a->cos || !a->sin || a->T < 1) return KATA_ERR_INVALID;
+    if (a->rope == 1 && a->R != a->D) return KATA_ERR_SHAPE;
+    if (a->rope == 2 && (a->R < 16 || a->R % 16 || a->D % a->R)) return KATA_ERR_SHAPE;
+  }
+  if (a->K > 0 && !a->conv_w) return KATA_ERR_INVALID;
+  const int C = (a->HQ + a->H) * a->D + a->H * a->Dv;
+  if (B > 1 && ldx < C) return KATA_ERR_SHAPE;
+  if (B == 0) return KATA_OK;
+  if (!x || !positions || !q || !k || !v || (a->K > 1 && !ring)) return KATA_ERR_INVALID;
+  auto al = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; };
+  if (!al(x) || !al(q) || !al(k) || !al(v) || (a->K > 1 && !al(ring)) || ldx % (a->dtype == KATA_DTYPE_F32 ? 4 : 8))
+    return KATA_ERR_ALIGN;
+  StepParams p;
+  p.x = x;
+  p.pos = reinterpret_cast<const long long*>(positions);
+  p.ring = ring;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.conv_w = a->conv_w;
+  p.qw = a->q_weight;
+  p.kw = a->k_weight;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.ldx = ldx;
+  p.B = static_cast<int>(B);
+  p.HQ = a->HQ;
+  p.H = a->H;
+  p.D = a->D;
+  p.Dv = a->Dv;
+  p.norm_q = a->norm_q;
+  p.norm_k = a->norm_k;
+  p.rope = a->rope;
+  p.R = a->R;
+  p.T = a->T;
+  p.eps_q = a->eps_q;
+  p.eps_k = a->eps_k;
+  int lph = 1;
+  while (lph * 8 < std::max(a->D, a->Dv)) lph *= 2;
+  p.lph = lph;
+  // more sequences than that per CTA once the grid fills the GPU several times over
+  const long long ctas = ((a->HQ + 2ll * a->H) * lph + kQT - 1) / kQT * B;
+  p.rows = static_cast<int>(std::max<long long>(std::min<long long>(8, ctas / (148 * 8)), (B + 65534) / 65535));
+  p.rows = std::max(p.rows, 1);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a->dtype == KATA_DTYPE_BF16)
+    launch_step<__nv_bfloat16>(p, a->K, st);
+  else if (a->dtype == KATA_DTYPE_F16)
+    launch_step<__half>(p, a->K, st);
+  else
+    launch_step<float>(p, a->K, st);
+  return from_cuda(cudaGetLastError());
+}

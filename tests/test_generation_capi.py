@@ -1,0 +1,109 @@
+"""The C entries of the generation operators refuse bad arguments on the host (no GPU is touched), and
+their Python fronts refuse CPU tensors."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from linatt_b200 import _lib
+
+
+@pytest.fixture(scope="module")
+def L():
+    from linatt_b200 import build
+
+    build.build()
+    return _lib.lib()
+
+
+def w4(**kw):
+    return _lib.W4WeightArgs(**{**dict(codes=16, scales=16, N=32, K=128, group=64, dtype=1, gated=0), **kw})
+
+
+def test_w4_layout_sizes(L):
+    def sizes(**kw):
+        s = [ctypes.c_size_t() for _ in range(3)]
+        assert L.kata_w4_layout(w4(**kw), *s) == 0
+        return [v.value for v in s]
+
+    # tiles of 16 rows, steps of 128 k: 1 KB of codes a step, 16 scales a group
+    assert sizes() == [2 * 1024, 2 * 2 * 16 * 2, 2 * 2 * 16]
+    assert sizes(N=33, K=129, group=32, dtype=0) == [3 * 2 * 1024, 3 * 8 * 16 * 4, 3 * 8 * 16]
+    assert sizes(N=34, K=700, group=256, gated=1) == [3 * 6 * 1024, 3 * 3 * 16 * 2, 3 * 3 * 16]
+    assert L.kata_w4_layout(w4(), None, None, None) == 0
+
+
+def test_w4_refusals(L):
+    ok = (16, 128, 16, 32, 1, None, None)
+    assert L.kata_w4_linear(None, *ok) == -1
+    assert L.kata_w4_linear(w4(dtype=3), *ok) == -2
+    for bad in (dict(group=0), dict(group=16), dict(group=96), dict(group=130), dict(N=0), dict(K=0),
+                dict(N=31, gated=1), dict(N=1 << 25)):
+        assert L.kata_w4_linear(w4(**bad), *ok) == -3, bad
+    assert L.kata_w4_linear(w4(gated=2), *ok) == -1
+    assert L.kata_w4_linear(w4(codes=None), *ok) == -1
+    assert L.kata_w4_linear(w4(codes=24), *ok) == -4
+    assert L.kata_w4_linear(w4(zeros=24), *ok) == -4
+    assert L.kata_w4_linear(w4(), None, 128, 16, 32, 1, None, None) == -1
+    assert L.kata_w4_linear(w4(), 17, 128, 16, 32, 1, None, None) == -4
+    assert L.kata_w4_linear(w4(), 16, 127, 16, 32, 2, None, None) == -3
+    assert L.kata_w4_linear(w4(), 16, 128, 16, 31, 2, None, None) == -3
+    assert L.kata_w4_linear(w4(), 16, 128, 16, 32, -1, None, None) == -3
+    assert L.kata_w4_linear(w4(), None, 128, None, 32, 0, None, None) == 0  # no rows: nothing to do
+    assert L.kata_w4_pack(None, 16, None, w4(), None) == -1
+    assert L.kata_w4_pack(16, 16, 16, w4(), None) == -1  # zeros without a place for them
+    assert L.kata_w4_pack(16, 16, None, w4(scales=20), None) == -4
+
+
+def test_qkv_step_refusals(L):
+    def step(B=1, x=16, ldx=128, pos=16, ring=16, q=16, k=16, v=16, **kw):
+        a = _lib.QkvStepArgs(**{**dict(conv_w=16, dtype=1, HQ=2, H=1, D=32, Dv=32, K=4), **kw})
+        return L.kata_qkv_step(a, x, ldx, pos, ring, q, k, v, B, None)
+
+    assert L.kata_qkv_step(None, 16, 128, 16, 16, 16, 16, 16, 1, None) == -1
+    assert step(dtype=5) == -2
+    for bad in (dict(H=0), dict(HQ=3, H=2), dict(D=0), dict(D=12), dict(D=264), dict(Dv=4), dict(B=-1)):
+        assert step(**bad) == -3, bad
+    assert step(K=5) == -8
+    for bad in (dict(norm_q=3), dict(rope=3), dict(rope=1, R=32), dict(conv_w=None), dict(x=None), dict(pos=None),
+                dict(ring=None), dict(v=None)):
+        assert step(**bad) == -1, bad
+    assert step(rope=1, R=16, cos=16, sin=16, T=4) == -3
+    assert step(rope=2, R=24, cos=16, sin=16, T=4) == -3
+    for bad in (dict(x=8), dict(q=8), dict(ring=8), dict(ldx=132)):
+        assert step(**bad) == -4, bad
+    assert step(B=2, ldx=120) == -3
+    assert step(B=0) == 0
+
+
+def test_sample_refusals(L):
+    def sample(**kw):
+        a = dict(logits=16, u=16, token=16, logprob=16, ld=100, B=2, V=100, dtype=1, temperature_all=1.0, top_p_all=1.0)
+        return L.kata_sample(_lib.SampleArgs(**{**a, **kw}), None)
+
+    assert L.kata_sample(None, None) == -1
+    assert sample(dtype=9) == -2
+    for bad in (dict(V=0), dict(V=(1 << 22) + 1), dict(B=-1), dict(ld=99)):
+        assert sample(**bad) == -3, bad
+    for bad in (dict(logits=None), dict(u=None), dict(token=None), dict(logprob=None)):
+        assert sample(**bad) == -1, bad
+    assert sample(logits=17) == -4
+    assert sample(B=0) == 0
+
+
+def test_fronts_refuse_cpu_tensors():
+    from linatt_b200.quant import W4Weight, quantize_w4
+    from linatt_b200.qkv_step import QKVStep
+    from linatt_b200.sampling import sample_tokens
+
+    with pytest.raises(RuntimeError):
+        W4Weight(torch.zeros(4, 4, dtype=torch.int32), torch.ones(4, 1), in_features=32, group_size=32)
+    with pytest.raises(RuntimeError):
+        quantize_w4(torch.zeros(4, 32))
+    with pytest.raises(RuntimeError):
+        QKVStep(num_heads=1, head_k_dim=8, head_v_dim=8, conv_weight=torch.zeros(24, 4))
+    with pytest.raises(RuntimeError):
+        sample_tokens(torch.zeros(2, 10), torch.zeros(2))
