@@ -560,24 +560,22 @@ KATA_API int kata_add_rmsnorm_bwd(const kata_add_rmsnorm_args* args, kata_stream
  *   W[n,k] = scale[n, k/group] * (code[n,k] - zero[n, k/group]),   codes 0..15, zero 8 when not given,
  * and, for a gated weight (gate rows 0..N/2-1, up rows N/2..N-1), y = silu(gate) * up with N/2 columns.
  * The codes and scales are exact in the products, which are summed in fp32 per group; only y is rounded.
- * `codes`, `scales` and `zeros` are in this library's tile layout, written once by kata_w4_pack (16-byte
- * aligned buffers of the sizes that kata_w4_layout gives).  group: 32, 64 or a multiple of 128.
- * dtype is that of x, y and the scales (f32 too: x is then used in full, as three bf16 parts).
+ * `data` is in this library's tile layout, written once by kata_w4_pack into kata_w4_bytes() bytes, 16-byte
+ * aligned.  group: 32, 64 or a multiple of 128.  dtype is that of x, y and the scales (fp32 x is used in full).
  * No counterpart in the reference, whose layers keep 16- or 32-bit weights.
  * ------------------------------------------------------------------------------------------- */
 typedef struct {
-  const void* codes;   /* from kata_w4_pack */
-  const void* scales;  /* from kata_w4_pack, dtype */
-  const void* zeros;   /* from kata_w4_pack, or NULL: all 8 */
+  const void* data;    /* from kata_w4_pack */
   int N, K, group, dtype;
   int gated;           /* 1: rows are [gate; up], y has N/2 columns */
+  int zeros;           /* 1: the groups have zero points of their own */
 } kata_w4_weight;
 
-/* Bytes of the three laid-out buffers (each may be NULL) for a weight of these sizes; KATA_OK or an error. */
-KATA_API int kata_w4_layout(const kata_w4_weight* w, size_t* code_bytes, size_t* scale_bytes, size_t* zero_bytes);
-/* Lays out a row-major quantised weight: packed (N, 4 ceil(K/32)) int32, code k of a row in bits
- * 4 (k % 8) .. +3 of word k / 8 (codes past K are ignored); scales (N, ceil(K/group)) dtype; zeros
- * (N, ceil(K/group)) uint8 in 0..15, or NULL.  Writes all bytes of the three buffers. */
+/* Bytes of the laid-out weight (data itself is not read); 0 for sizes that are refused. */
+KATA_API size_t kata_w4_bytes(const kata_w4_weight* w);
+/* Lays out a row-major quantised weight into w->data: packed (N, 4 ceil(K/32)) int32, code k of a row in
+ * bits 4 (k % 8) .. +3 of word k / 8 (codes past K are ignored); scales (N, ceil(K/group)) dtype; zeros
+ * (N, ceil(K/group)) uint8 in 0..15, or NULL when w->zeros is 0. */
 KATA_API int kata_w4_pack(const void* packed, const void* scales, const void* zeros, const kata_w4_weight* w,
                           kata_stream_t stream);
 /* y (rows, ldy) = x (rows, ldx) W^T; row strides in elements, both with contiguous columns.  x of any

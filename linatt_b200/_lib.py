@@ -132,8 +132,8 @@ class AddRmsNormArgs(ctypes.Structure):
 
 class W4WeightArgs(ctypes.Structure):
     _fields_ = [
-        ("codes", c_void_p), ("scales", c_void_p), ("zeros", c_void_p),
-        ("N", c_int), ("K", c_int), ("group", c_int), ("dtype", c_int), ("gated", c_int),
+        ("data", c_void_p), ("N", c_int), ("K", c_int), ("group", c_int), ("dtype", c_int), ("gated", c_int),
+        ("zeros", c_int),
     ]
 
 
@@ -253,9 +253,8 @@ def lib() -> ctypes.CDLL:
             L.kata_add_rmsnorm_bwd_workspace_bytes.restype = c_size_t
             L.kata_add_rmsnorm_bwd_workspace_bytes.argtypes = [ctypes.POINTER(AddRmsNormArgs)]
             P_W4 = ctypes.POINTER(W4WeightArgs)
-            P_SZ = ctypes.POINTER(c_size_t)
-            L.kata_w4_layout.restype = c_int
-            L.kata_w4_layout.argtypes = [P_W4, P_SZ, P_SZ, P_SZ]
+            L.kata_w4_bytes.restype = c_size_t
+            L.kata_w4_bytes.argtypes = [P_W4]
             L.kata_w4_pack.restype = c_int
             L.kata_w4_pack.argtypes = [c_void_p, c_void_p, c_void_p, P_W4, c_void_p]
             L.kata_w4_linear.restype = c_int
@@ -297,7 +296,8 @@ def require_cuda(*ts: torch.Tensor | None) -> torch.device:
 
 
 def stream_handle(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # the handle alone: building a torch.cuda.Stream object around it costs 2 us of a small call's 7
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 class _Stay:

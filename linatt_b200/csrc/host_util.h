@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kata_b200.h"
 
 namespace kata {
@@ -27,6 +29,18 @@ inline CUtensorMapSwizzle swizzle_enum(int bytes) {
 // strides are in bytes for dims 1..rank-1.  Returns a KATA_ERR_* code.
 int encode_tmap_16bit(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                       const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes);
+
+// Lets a kernel use up to `bytes` of dynamic shared memory, once per kernel and device (the call costs
+// as much as a launch); `done` is the kernel's own word of the devices seen.
+inline int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return KATA_ERR_CUDA;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return KATA_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return KATA_ERR_CUDA;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return KATA_OK;
+}
 
 inline int from_cuda(cudaError_t e) { return e == cudaSuccess ? KATA_OK : KATA_ERR_CUDA; }
 

@@ -4,11 +4,11 @@
 // Layout (written once by kata_w4_pack).  Rows go in tiles of 16, k in steps of 128; a tile's steps and
 // the tiles themselves are contiguous, so that a run of work is one run of memory.  A step of a tile is
 // 1 KB: [row half][lane][block of 32 k] words of 8 codes, lane = 4 (row % 8) + q holding codes 8q..8q+7
-// of each block, which are exactly the lane's A-fragment values of mma.m16n8k16 (two MMAs a block, the
-// k slots of an MMA being codes 8q + 4j + {0,1} and {2,3} of the four lanes q).  Nibble i of a word is
-// code 2i and nibble i + 4 code 2i + 1, so that (word >> 4i) & 0x000f000f is a pair of neighbours.
-// Scales (and zeros) follow as [tile][group][16 rows].  A gated weight's tile holds 8 gate rows and the
-// 8 up rows that belong to them, so that both sums of an output end in the same lane.
+// of each block: byte j of a word has code j in its low and code j + 4 in its high nibble, so that
+// word & 0x0f0f0f0f and (word >> 4) & 0x0f0f0f0f are four neighbours as bytes -- as they are, the lane's
+// A-fragment registers of mma.m16n8k32 on bytes (k slots 4q..4q+3 and 16+4q.. being codes 8q.. and 8q+4..).
+// The step's scales, [group][16 rows], and zeros follow in the same record (a group of several steps is
+// stored in each of them), so that a run of steps is one bulk copy.  A gated weight's tile holds 8 gate rows and the 8 up rows that belong to them.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -18,13 +18,14 @@
 namespace kata {
 namespace {
 
+constexpr int kMaxSmem = 232448;  // dynamic shared memory a CTA may have
 constexpr int kStepBytes = 1024;  // codes of 16 rows x 128 k
 
 struct W4Geom {
   int tiles, steps;  // row tiles, steps of 128 k
-  int gps;           // groups a step spans (4, 2 or 1)
-  int spg;           // steps a group spans (1 unless group > 128)
-  int groups;        // groups stored per tile: every step's run is whole
+  int gps;           // groups of a step (4, 2 or 1; a group of several steps is stored once for each)
+  int side;          // bytes of a step's scales and zeros
+  int rec;           // bytes of a step
 };
 
 inline W4Geom w4_geom(const kata_w4_weight* w) {
@@ -32,8 +33,8 @@ inline W4Geom w4_geom(const kata_w4_weight* w) {
   g.tiles = w->gated ? (w->N / 2 + 7) / 8 : (w->N + 15) / 16;
   g.steps = (w->K + 127) / 128;
   g.gps = w->group < 128 ? 128 / w->group : 1;
-  g.spg = w->group > 128 ? w->group / 128 : 1;
-  g.groups = w->group <= 128 ? g.steps * g.gps : (g.steps + g.spg - 1) / g.spg;
+  g.side = g.gps * 16 * ((w->dtype == KATA_DTYPE_F32 ? 4 : 2) + (w->zeros ? 1 : 0));
+  g.rec = kStepBytes + g.side;
   return g;
 }
 
@@ -47,386 +48,519 @@ __host__ __device__ inline int w4_row(int t, int r, int N, int gated) {
   return n < N / 2 ? n + (r >> 3) * (N / 2) : -1;
 }
 
-// One thread per word of the laid-out codes; then the scales and zeros of each (tile, group, row).
-__global__ void __launch_bounds__(256) w4_pack_codes_kernel(const uint32_t* __restrict__ packed,
-                                                            uint32_t* __restrict__ codes, int N, int K, int gated,
-                                                            int steps, long long words) {
-  const int wpr = 4 * ((K + 31) / 32);  // words a row of the input has
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < words; i += gridDim.x * 256ll) {
-    const int b = i & 3, lane = (i >> 2) & 31, half = (i >> 7) & 1;
-    const long long f = i >> 8;
-    const int step = static_cast<int>(f % steps), t = static_cast<int>(f / steps);
-    const int n = w4_row(t, half * 8 + (lane >> 2), N, gated);
-    const int src = step * 16 + b * 4 + (lane & 3);
-    uint32_t v = 0x88888888u;
-    if (n >= 0 && src < wpr) v = packed[static_cast<size_t>(n) * wpr + src];
-    uint32_t o = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      o |= ((v >> (8 * j)) & 15u) << (4 * j);
-      o |= ((v >> (8 * j + 4)) & 15u) << (4 * j + 16);
-    }
-    codes[i] = o;
-  }
-}
-
+// One warp per record: its codes, then its scales and zeros.
 template <typename S>
-__global__ void __launch_bounds__(256) w4_pack_scales_kernel(const S* __restrict__ scales, S* __restrict__ out, int N,
-                                                             int G, int gated, int groups, long long n_out, S fill) {
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n_out; i += gridDim.x * 256ll) {
-    const long long f = i >> 4;
-    const int g = static_cast<int>(f % groups), t = static_cast<int>(f / groups);
-    const int n = w4_row(t, static_cast<int>(i & 15), N, gated);
-    out[i] = (n >= 0 && g < G) ? scales[static_cast<size_t>(n) * G + g] : fill;
+__global__ void __launch_bounds__(256) w4_pack_kernel(const uint32_t* __restrict__ packed, const S* __restrict__ scales,
+                                                      const uint8_t* __restrict__ zeros, unsigned char* __restrict__ data,
+                                                      int N, int K, int group, int gated, W4Geom g) {
+  const int wpr = 4 * ((K + 31) / 32);  // words a row of the input has
+  const int G = (K + group - 1) / group, lane = threadIdx.x & 31;
+  const long long records = static_cast<long long>(g.tiles) * g.steps;
+  for (long long f = blockIdx.x * 8ll + (threadIdx.x >> 5); f < records; f += gridDim.x * 8ll) {
+    const int step = static_cast<int>(f % g.steps), t = static_cast<int>(f / g.steps);
+    unsigned char* rec = data + f * g.rec;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int n = w4_row(t, half * 8 + (lane >> 2), N, gated);
+      uint32_t o[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int src = step * 16 + b * 4 + (lane & 3);
+        const uint32_t v = n >= 0 && src < wpr ? packed[static_cast<size_t>(n) * wpr + src] : 0x88888888u;
+        o[b] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[b] |= ((v >> (4 * j)) & 15u) << (8 * j) | ((v >> (4 * j + 16)) & 15u) << (8 * j + 4);
+      }
+      reinterpret_cast<uint4*>(rec)[half * 32 + lane] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    for (int i = lane; i < g.gps * 16; i += 32) {
+      const int n = w4_row(t, i & 15, N, gated), gr = min((step * 128 + (i >> 4) * (128 / g.gps)) / group, G);
+      const bool live = n >= 0 && gr < G;
+      reinterpret_cast<S*>(rec + kStepBytes)[i] = live ? scales[static_cast<size_t>(n) * G + gr] : S(0);
+      if (zeros) rec[kStepBytes + g.gps * 16 * sizeof(S) + i] = live ? zeros[static_cast<size_t>(n) * G + gr] : 8;
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------
 // Streaming kernel: few rows of x, the codes read once from HBM.
+//
+// Turning codes into 16-bit floats costs 11 instructions a word and bounds such a kernel at half the HBM
+// rate (measured: 1 x 8192 x 32768 in 36 us against 21 us for the bytes).  Bytes cost 3.  So x becomes
+// whole numbers: the 128 values of a row's step are scaled by a power of two to |v| <= 2^22 (fp32: 2^30)
+// and split into 3 (4) signed base-256 digits, each a column of the product, whose sums over a group are
+// exact in 32 bits.  A value keeps all bits down to 2^-22 (2^-30) of the largest of its 128, and is off by
+// half of that below: less than the fp32 sums over the groups lose.  A group's sum of (code - 8) times a
+// digit is below 2^22, so it is accumulated on top of the bits of 1.5 2^23 and is a float as it stands;
+// -8 sum(digits) is part of that start.  Infinities and NaN are left out of the digits and added to the
+// sums of their row at the end.
 // ------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+__device__ __forceinline__ void imma16832(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Codes to 16-bit floats: a nibble ORed into the mantissa of 128 (bf16) or 1024 (f16) is 128 + code or
-// 1024 + code exactly; from there one fused multiply-add leaves unit (code - zero) exactly.  With bf16
-// the unit is 2^-10: a group's sum of unscaled products stays finite for every finite x.  f16 values are
-// too small to come near the end of fp32 (unit 1).  The scale takes the unit back.
-template <typename T>
-struct Magic;
-template <>
-struct Magic<__nv_bfloat16> {
-  static constexpr uint32_t base = 0x43004300u;   // 128
-  static constexpr uint32_t unit = 0x3a803a80u;   // 2^-10
-  static constexpr float back = 1024.f;
-  // -(128 + zero) 2^-10
-  static __device__ __forceinline__ uint32_t offset(uint32_t zero) {
-    const __nv_bfloat162 v = __float2bfloat162_rn(-(128.f + static_cast<float>(zero)) * (1.f / 1024.f));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b) {
-    const uint32_t u = unit;
-    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&u),
-                                     *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
-template <>
-struct Magic<__half> {
-  static constexpr uint32_t base = 0x64006400u;   // 1024
-  static constexpr float back = 1.f;
-  // -(1024 + zero)
-  static __device__ __forceinline__ uint32_t offset(uint32_t zero) { return 0xe400e400u + 0x00010001u * zero; }
-  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b) {
-    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
-template <typename T>
-__device__ __forceinline__ uint32_t dequant_pair(uint32_t word, int i, uint32_t offset) {
-  return Magic<T>::fma2(((word >> (4 * i)) & 0x000f000fu) | Magic<T>::base, offset);
-}
-
-// An fp32 value as three bf16 parts, each the leading 8 bits of what is left: exact together, and no
-// part overflows.  Infinities and NaN stay in the first part.
-__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
-  const float a = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  const bool fin = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
-  const float r = fin ? x - a : 0.f;
-  const float b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-  p[0] = __float2bfloat16_rn(fin ? a : x);
-  p[1] = __float2bfloat16_rn(b);
-  p[2] = __float2bfloat16_rn(r - b);
 }
 
 struct W4Params {
-  const unsigned char* codes;
-  const unsigned char* scales;
-  const unsigned char* zeros;
+  const unsigned char* data;
   const void* x;
   void* y;
   long long ldx, ldy;
-  int rows, N, K, gated;
+  int* status;
+  int rows, N, K, gated, zeros;
   W4Geom g;
-  int tpb;          // row tiles a CTA works on at once (its partial sums are kept in shared memory)
+  int tiles_q, tiles_r;  // tiles of a CTA, and how many CTAs have one more
+  int chunks, slab_rows;
+  int tpb;          // row tiles a CTA works on at once (their sums are kept in shared memory)
   int chunk_steps;  // steps of k whose x is in shared memory at once
-  int stage_bytes;
+  int vec;          // rows of x start on 16-byte boundaries
+  int wpr;          // warps that a row of x is staged by
+  uint32_t by_steps, by_rows, by_wpr;  // reciprocals of chunk_steps, the rows of a slab and wpr
 };
 
-constexpr int kWarps = 8;
-constexpr int kDepth = 6;  // steps in flight per warp
+// n / d through the reciprocal r = ceil(2^32 / d), for n d < 2^32 (a division costs 100 cycles of a call's 3000)
+inline uint32_t recip(uint32_t d) { return d == 1 ? 0 : static_cast<uint32_t>((0x100000000ull + d - 1) / d); }
+__device__ __forceinline__ int div_by(int n, uint32_t r) { return r ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), r)) : n; }
 
-// T: operand type of the products; X: type of x, y and the scales (float: PARTS = 3 columns a row).
-// NT: tiles of 8 columns.  GPS: groups per step.
-template <typename T, typename X, int NT, int GPS, bool ZERO>
-__global__ void __launch_bounds__(kWarps * 32) w4_stream_kernel(const W4Params p) {
-  constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
+constexpr int kWarps = 16;
+// steps per copy, at most: fewer where the scales are many, so that the rings leave room for x
+constexpr int unit_of(int side_bytes) { return side_bytes > 96 ? 2 : 4; }
+constexpr int kDepth = 2;  // copies in flight per warp
+constexpr int kMagicBits = 0x4b400000;  // 1.5 2^23
+constexpr float kMagic = 12582912.f;
+
+template <typename X>
+struct Digits {
+  static constexpr int N = sizeof(X) == 4 ? 4 : 3;
+  static constexpr int bits = sizeof(X) == 4 ? 30 : 22;
+};
+
+// Eight neighbours of a row of x as they are in memory (zeros past its end)
+template <typename X>
+struct Raw8 {
+  uint4 w[sizeof(X) / 2];
+  __device__ __forceinline__ void load(const X* src, int left, bool vec) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(X) / 2); ++i) w[i] = make_uint4(0, 0, 0, 0);
+    if (vec && left >= 8) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(X) / 2); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    } else if (left > 0) {
+      X* e = reinterpret_cast<X*>(w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) e[j] = src[j];
+    }
+  }
+  __device__ __forceinline__ float operator[](int j) const { return to_f32<X>(reinterpret_cast<const X*>(w)[j]); }
+};
+__device__ __forceinline__ bool finite_bits(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// scale[n, k / g] (code - zero) of the tile's row r at k, from the layout
+template <typename X>
+__device__ float w4_at(const W4Params& p, int t, int r, int k) {
+  const unsigned char* rec = p.data + (static_cast<long long>(t) * p.g.steps + k / 128) * p.g.rec;
+  const int kk = k % 128, b = kk / 32, q = (kk % 32) / 8, j = kk % 8;
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + (r >> 3) * 512 + ((r & 7) * 4 + q) * 16 + b * 4);
+  const int code = (w >> ((j & 3) * 8 + (j >> 2) * 4)) & 15;
+  const int gi = kk / (128 / p.g.gps) * 16 + r;
+  const int zero = p.zeros ? rec[kStepBytes + p.g.gps * 16 * sizeof(X) + gi] & 15 : 8;
+  return to_f32<X>(reinterpret_cast<const X*>(rec + kStepBytes)[gi]) * static_cast<float>(code - zero);
+}
+
+// NT: tiles of 8 columns (digits of rows).  GPS: groups per step.
+//
+// A CTA owns a run of row tiles; their (tile, unit of k) pairs are one list that the warps split evenly, so
+// no warp waits for another until the end.  A warp streams its run through a ring of its own, filled by one
+// lane's bulk copies.  Its part of a tile goes to shared memory when the tile ends, and the sums over warps
+// are taken in their order at the end.
+template <typename X, int NT, int GPS, bool ZERO>
+__global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Params p) {
+  constexpr int ND = Digits<X>::N;
   constexpr int COLS = 8 * NT;
-  constexpr int ROWS = COLS / PARTS;  // rows of x a CTA takes
+  constexpr int ROWS = COLS / ND;                             // rows of x a CTA takes
+  constexpr int SB = GPS * 16 * static_cast<int>(sizeof(X));  // scale bytes of a step
+  constexpr int ZB = ZERO ? GPS * 16 : 0;
+  constexpr int kUnit = unit_of(SB + ZB);
+  constexpr int REC = kStepBytes + SB + ZB;
+  constexpr int STAGE = kUnit * REC;
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint64_t bars[kWarps][kDepth];
+  __shared__ int abort_flag;
+  __shared__ int row_odd[ROWS];  // whether a row has infinities or NaN
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row0 = blockIdx.y * ROWS;
-  const int nrow = min(ROWS, p.rows - row0), ncol = nrow * PARTS;
-  const int kc = p.chunk_steps * 128;
-  const int pitch = kc + 32;  // 64 bytes more than a multiple of 256: the eight 16-byte reads of a quarter warp
-                              // (two columns, four q) fall on all 32 banks
-  T* xs = reinterpret_cast<T*>(smem);
-  unsigned char* ring = smem + static_cast<size_t>(min(COLS, p.rows * PARTS)) * pitch * sizeof(T);
-  float* red = reinterpret_cast<float*>(ring + kWarps * kDepth * p.stage_bytes);
-  unsigned char* myring = ring + warp * kDepth * p.stage_bytes;
-  const uint32_t myring_s = smem_u32(myring);
-
-  // this CTA's tiles, as even as whole tiles allow
-  const int t_lo = static_cast<int>(static_cast<long long>(p.g.tiles) * blockIdx.x / gridDim.x);
-  const int t_hi = static_cast<int>(static_cast<long long>(p.g.tiles) * (blockIdx.x + 1) / gridDim.x);
-  const int g = lane >> 2, q = lane & 3;
-  const int chunks = (p.g.steps + p.chunk_steps - 1) / p.chunk_steps;
+  const int nrow = min(ROWS, p.rows - row0), ncol = nrow * ND;
+  const int pitch = p.chunk_steps * 128 + 16;  // bytes of a column
+  unsigned char* ring = smem;
+  float* red = reinterpret_cast<float*>(smem + kWarps * kDepth * STAGE);
+  // of a group and two neighbouring columns: where their sums start (ZERO: the sums of the digits), their units
+  int4* start = reinterpret_cast<int4*>(red + (p.tpb + kWarps - 1) * 16 * COLS);  // [group][COLS / 2]
+  unsigned char* xs = reinterpret_cast<unsigned char*>(start + p.chunk_steps * GPS * COLS / 2);  // [column][step][q][b][8]
+  // A thread's first items of x, eight values each, are on their way before the codes: behind those they
+  // would wait for as long as the copies in flight take (3 us measured)
+  const int sr = div_by(warp, p.by_wpr), si = (warp - sr * p.wpr) * 32 + lane, sn = p.wpr * 32;
   const X* x = static_cast<const X*>(p.x) + row0 * p.ldx;
-  const int bcol = min(g, ncol - 1);  // columns past the last hold what nobody reads
+  const X* xr = x + sr * p.ldx;
+  const int x_steps = min(p.chunk_steps, p.g.steps);
+  auto load_x = [&](Raw8<X>& v, int s0, int ns, int i) {
+    v.load(xr + s0 * 128 + i * 8, sr < nrow && i < ns * 16 ? p.K - s0 * 128 - i * 8 : 0, p.vec);
+  };
+  Raw8<X> x0, x1;
+  load_x(x0, 0, x_steps, si);
+  load_x(x1, 0, x_steps, si + sn);
+  if (tid == 0) abort_flag = 0;
+  if (tid < ROWS) row_odd[tid] = 0;
+  if (lane == 0) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) mbar_init(&bars[warp][d], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const WaitCtx wait{p.status, &abort_flag};
+
+  const int t_lo = p.tiles_q * blockIdx.x + min(static_cast<int>(blockIdx.x), p.tiles_r);
+  const int t_hi = t_lo + p.tiles_q + (static_cast<int>(blockIdx.x) < p.tiles_r ? 1 : 0);
+  const int chunks = p.chunks;
+  const int spt = p.chunk_steps;  // steps a tile has in a chunk, the same in every chunk (the last one's surplus is
+                                  // skipped), so that a warp's tiles are too
+  const int g = lane >> 2, q = lane & 3;
+  unsigned char* myring = ring + warp * kDepth * STAGE;
+  uint32_t phase = 0;  // of each stage's barrier, one bit a stage
+  bool ok = true;
 
   for (int tb = t_lo; tb < t_hi; tb += p.tpb) {
     const int nt = min(p.tpb, t_hi - tb);
-    const int total = nt * p.chunk_steps;
-    const int f_lo = total * warp / kWarps, f_hi = total * (warp + 1) / kWarps;
+    const int total = nt * spt;
+    const int per = (total + kWarps - 1) / kWarps;  // steps of a warp
+    const int f_lo = min(total, warp * per), f_hi = min(total, f_lo + per);
     for (int ch = 0; ch < chunks; ++ch) {
       const int s0 = ch * p.chunk_steps;
       const int ns = min(p.chunk_steps, p.g.steps - s0);
-      if (ch > 0 || (tb > t_lo && chunks > 1)) __syncthreads();  // the chunk before is no longer read
-      if (tb == t_lo || chunks > 1) {
-        const int k0 = s0 * 128;
-        const bool vec = sizeof(X) == 2 && (p.ldx % 8) == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0;
-        for (int i = tid; i < nrow * (kc / 8); i += kWarps * 32) {
-          const int r = i / (kc / 8), k = (i - r * (kc / 8)) * 8;
-          const X* src = x + r * p.ldx + k0 + k;
-          if (vec && k0 + k + 8 <= p.K) {
-            *reinterpret_cast<uint4*>(xs + r * pitch + k) = *reinterpret_cast<const uint4*>(src);
-          } else {
+      // The copies follow the warp's steps in memory: with x in one chunk its whole run is contiguous, else
+      // the part of each tile.  `is` is the step of the tile, `fi` the place in the list.
+      const bool whole = chunks == 1;
+      const int tile_lo = div_by(f_lo, p.by_steps), step_lo = f_lo - tile_lo * spt;
+      int is = step_lo, fi = f_lo, ist = 0;
+      auto copy_len = [&](int f, int st) { return min(min(kUnit, f_hi - f), whole ? kUnit : ns - st); };
+      const long long first = static_cast<long long>(tb + tile_lo) * p.g.steps + s0 + is;
+      const unsigned char* src = p.data + first * REC;
+      auto issue = [&]() {
+        if (!whole && is >= ns) {  // on to the next tile
+          src += (p.g.steps - is) * REC;
+          fi += spt - is;
+          is = 0;
+        }
+        if (fi >= f_hi || !ok) return;
+        const int n = copy_len(fi, is);
+        if (lane == 0) {
+          uint64_t* bar = &bars[warp][ist];
+          mbar_arrive_expect_tx(bar, n * REC);
+          bulk_load(myring + ist * STAGE, src, n * REC, bar);
+        }
+        ist = ist + 1 == kDepth ? 0 : ist + 1;
+        fi += n;
+        is += n;
+        src += n * REC;
+      };
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const X v = k0 + k + j < p.K ? src[j] : from_f32<X>(0.f);
-              if constexpr (PARTS == 1) {
-                xs[r * pitch + k + j] = v;
-              } else {
-                __nv_bfloat16 s3[3];
-                split3(v, s3);
+      for (int d = 0; d < kDepth; ++d) issue();
+
+      if ((tb == t_lo && ch == 0) || !whole) {
+        if (ch > 0 || tb > t_lo) {
+          __syncthreads();  // the chunk before is no longer read
+          load_x(x0, s0, ns, si);
+          load_x(x1, s0, ns, si + sn);
+        }
+        const int items = (ns * 16 + 31) / 32 * 32;  // whole warps, since lanes share a step
+#pragma unroll 1
+        for (int i = sr < nrow ? si : items; i < items; i += sn) {
+          const Raw8<X> v = x0;
+          x0 = x1;
+          load_x(x1, s0, ns, i + 2 * sn);
+          uint32_t m = 0;
 #pragma unroll
-                for (int c = 0; c < 3; ++c) xs[(r * 3 + c) * pitch + k + j] = s3[c];
-              }
+          for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+          const bool odd = __any_sync(0xffffffffu, m >= 0x7f800000u);
+          if (odd) {
+            if (m >= 0x7f800000u) row_odd[sr] = 1;
+            m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (finite_bits(v[j])) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+          }
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const int e = max(static_cast<int>(m >> 23), 30);  // |x| < 2^(e - 126)
+          const float up = __uint_as_float(static_cast<uint32_t>(Digits<X>::bits + 126 - e + 127) << 23);
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            // the bytes of (n + B) ^ B are the balanced digits of n (B has 0x80 in every byte but the top one)
+            constexpr uint32_t B = ND == 4 ? 0x808080u : 0x8080u;
+            int n = __float2int_rn(v[j] * up);
+            if (odd && !finite_bits(v[j])) n = 0;
+            w[j] = (static_cast<uint32_t>(n) + B) ^ B;
+          }
+          const int st = i >> 4, b = (i >> 2) & 3, iq = i & 3;
+          const bool live = i < ns * 16;
+          int unit = e + 1 - Digits<X>::bits;  // exponent bits of 2^(e - 126 - bits)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {  // byte d of each
+            const uint32_t sel = 0x0040u + 0x0011u * d;  // bytes d and 4 + d
+            const uint32_t lo = __byte_perm(__byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel), 0x5410);
+            const uint32_t hi = __byte_perm(__byte_perm(w[4], w[5], sel), __byte_perm(w[6], w[7], sel), 0x5410);
+            const int col = sr * ND + d;
+            if (live) *reinterpret_cast<uint2*>(xs + col * pitch + st * 128 + iq * 32 + b * 8) = make_uint2(lo, hi);
+            int sum = __dp4a(static_cast<int>(lo), 0x01010101, __dp4a(static_cast<int>(hi), 0x01010101, 0));
+#pragma unroll
+            for (int o = 1; o < 16 / GPS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (live && (i & (16 / GPS - 1)) == 0) {
+              int* at = reinterpret_cast<int*>(start + (i / (16 / GPS)) * (COLS / 2) + (col >> 1)) + (col & 1);
+              at[0] = ZERO ? sum : kMagicBits - 8 * sum;
+              at[2] = unit << 23;
             }
+            unit += 8;
           }
         }
         __syncthreads();
       }
 
-      // this warp's run of (tile, step); `it`, `is` are where the next copy goes
-      int it = f_lo / p.chunk_steps, is = f_lo - it * p.chunk_steps;
-      int ct = it, cs = is;
-      int fi = f_lo;
-      auto issue = [&]() {
-        if (fi < f_hi && is < ns) {
-          const uint32_t dst = myring_s + ((fi - f_lo) % kDepth) * p.stage_bytes;
-          const long long f = static_cast<long long>(tb + it) * p.g.steps + s0 + is;
-          const unsigned char* src = p.codes + f * kStepBytes;
-          cp_async16(dst + lane * 16, src + lane * 16);
-          cp_async16(dst + 512 + lane * 16, src + 512 + lane * 16);
-          const long long gi = p.g.spg == 1 ? f * GPS : static_cast<long long>(tb + it) * p.g.groups + (s0 + is) / p.g.spg;
-          constexpr int SB = GPS * 16 * static_cast<int>(sizeof(X));  // scales of a step
+      int ct = tile_lo, cs = step_lo, cst = 0;
+      // columns past the last hold what nobody reads
+      const unsigned char* xl[NT];
 #pragma unroll
-          for (int o = 0; o < SB; o += 128)
-            if (o + lane * 4 < SB) cp_async4(dst + kStepBytes + o + lane * 4, p.scales + gi * 16 * sizeof(X) + o + lane * 4);
-          if (ZERO && lane < GPS * 4) cp_async4(dst + kStepBytes + SB + lane * 4, p.zeros + gi * 16 + lane * 4);
-        }
-        cp_async_commit();
-        ++fi;
-        if (++is == p.chunk_steps) {
-          is = 0;
-          ++it;
-        }
-      };
-#pragma unroll
-      for (int d = 0; d < kDepth - 1; ++d) issue();
-
+      for (int n = 0; n < NT; ++n) xl[n] = xs + min(n * 8 + g, ncol - 1) * pitch + q * 32;
+      const int4* sl = start + q;
       float acc[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-      for (int f = f_lo; f < f_hi; ++f) {
-        cp_async_wait<kDepth - 2>();
-        __syncwarp();  // every lane's copies of this step are in, and the step before is no longer read
-        issue();
-        if (cs < ns) {
-          const unsigned char* st = myring + ((f - f_lo) % kDepth) * p.stage_bytes;
-          const uint4 w0 = *reinterpret_cast<const uint4*>(st + lane * 16);
-          const uint4 w1 = *reinterpret_cast<const uint4*>(st + 512 + lane * 16);
-          const uint32_t wa[4] = {w0.x, w0.y, w0.z, w0.w}, wb[4] = {w1.x, w1.y, w1.z, w1.w};
-          const X* sc = reinterpret_cast<const X*>(st + kStepBytes);
-          const unsigned char* zp = st + kStepBytes + GPS * 16 * sizeof(X);
-          float part[NT][4];
-          uint32_t z0 = Magic<T>::offset(8), z1 = z0;
+      auto flush = [&]() {
+        // this warp's part of the tile: tiles and warps grow together along the list, so tile + warp is a
+        // slot of its own
+        float* slot = red + static_cast<size_t>(ct + warp) * 16 * COLS + g * COLS + 2 * q;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            if (b % (4 / GPS) == 0) {
-#pragma unroll
-              for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
-              if (ZERO) {
-                z0 = Magic<T>::offset(zp[(b * GPS / 4) * 16 + g] & 15u);
-                z1 = Magic<T>::offset(zp[(b * GPS / 4) * 16 + g + 8] & 15u);
-              }
-            }
-            uint32_t a[2][4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              a[j][0] = dequant_pair<T>(wa[b], 2 * j, z0);
-              a[j][1] = dequant_pair<T>(wb[b], 2 * j, z1);
-              a[j][2] = dequant_pair<T>(wa[b], 2 * j + 1, z0);
-              a[j][3] = dequant_pair<T>(wb[b], 2 * j + 1, z1);
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const int col = NT == 1 ? bcol : min(n * 8 + g, ncol - 1);
-              const uint4 xv = *reinterpret_cast<const uint4*>(xs + col * pitch + cs * 128 + b * 32 + q * 8);
-              mma16816(part[n], a[0], xv.x, xv.y, T());
-              mma16816(part[n], a[1], xv.z, xv.w, T());
-            }
-            if (b % (4 / GPS) == 4 / GPS - 1) {
-              const float s0f = to_f32<X>(sc[(b * GPS / 4) * 16 + g]) * Magic<T>::back;
-              const float s1f = to_f32<X>(sc[(b * GPS / 4) * 16 + g + 8]) * Magic<T>::back;
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                acc[n][0] = fmaf(s0f, part[n][0], acc[n][0]);
-                acc[n][1] = fmaf(s0f, part[n][1], acc[n][1]);
-                acc[n][2] = fmaf(s1f, part[n][2], acc[n][2]);
-                acc[n][3] = fmaf(s1f, part[n][3], acc[n][3]);
-              }
-            }
-          }
+        for (int n = 0; n < NT; ++n) {
+          float2* d0 = reinterpret_cast<float2*>(slot + n * 8);
+          float2* d1 = reinterpret_cast<float2*>(slot + 8 * COLS + n * 8);
+          *d0 = ch == 0 ? make_float2(acc[n][0], acc[n][1]) : make_float2(d0->x + acc[n][0], d0->y + acc[n][1]);
+          *d1 = ch == 0 ? make_float2(acc[n][2], acc[n][3]) : make_float2(d1->x + acc[n][2], d1->y + acc[n][3]);
+          acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
         }
-        if (++cs == p.chunk_steps || f + 1 == f_hi) {
-          // the tile's part of this warp: tiles and warps grow together along the run, so tile + warp
-          // is a slot of its own
-          float* slot = red + static_cast<size_t>(ct + warp) * 16 * COLS;
+      };
+      int f = f_lo;
+      if (cs >= ns) {  // starts in the last chunk's surplus
+        f += spt - cs;
+        cs = 0;
+        ++ct;
+      }
+      while (f < f_hi) {
+        const int n_steps = copy_len(f, cs);
+        ok = mbar_wait_w(&bars[warp][cst], (phase >> cst) & 1u, wait);
+        if (!ok) break;
+        phase ^= 1u << cst;
+        const unsigned char* stg = myring + cst * STAGE;
+        auto step = [&](int u) {
+          const unsigned char* rec = stg + u * REC;
+          const uint4 w0 = *reinterpret_cast<const uint4*>(rec + lane * 16);
+          const uint4 w1 = *reinterpret_cast<const uint4*>(rec + 512 + lane * 16);
+          const uint32_t wa[4] = {w0.x, w0.y, w0.z, w0.w}, wb[4] = {w1.x, w1.y, w1.z, w1.w};
+          const X* sc = reinterpret_cast<const X*>(rec + kStepBytes) + g;
+          const unsigned char* zp = rec + kStepBytes + SB + g;
+          uint32_t xb[NT][8];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
+            const uint4 x0 = *reinterpret_cast<const uint4*>(xl[n] + cs * 128);
+            const uint4 x1 = *reinterpret_cast<const uint4*>(xl[n] + cs * 128 + 16);
+            xb[n][0] = x0.x, xb[n][1] = x0.y, xb[n][2] = x0.z, xb[n][3] = x0.w;
+            xb[n][4] = x1.x, xb[n][5] = x1.y, xb[n][6] = x1.z, xb[n][7] = x1.w;
+          }
+          int part[NT][4];
+          int4 begin[NT];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float* d = slot + (g + (e >> 1) * 8) * COLS + n * 8 + 2 * q + (e & 1);
-              *d = ch == 0 ? acc[n][e] : *d + acc[n][e];
-              acc[n][e] = 0.f;
+          for (int b = 0; b < 4; ++b) {
+            constexpr int BPG = 4 / GPS;  // blocks of a group
+            const int gr = cs * GPS + b / BPG;
+            if (b % BPG == 0) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                begin[n] = sl[gr * (COLS / 2) + n * 4];
+                part[n][0] = part[n][2] = ZERO ? kMagicBits : begin[n].x;
+                part[n][1] = part[n][3] = ZERO ? kMagicBits : begin[n].y;
+              }
+            }
+            const uint32_t a[4] = {wa[b] & 0x0f0f0f0fu, wb[b] & 0x0f0f0f0fu, (wa[b] >> 4) & 0x0f0f0f0fu,
+                                   (wb[b] >> 4) & 0x0f0f0f0fu};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) imma16832(part[n], a, xb[n][2 * b], xb[n][2 * b + 1]);
+            if (b % BPG == BPG - 1) {
+              const float s0f = to_f32<X>(sc[(b / BPG) * 16]), s1f = to_f32<X>(sc[(b / BPG) * 16 + 8]);
+              float z0 = 0.f, z1 = 0.f;
+              if (ZERO) {
+                z0 = -static_cast<float>(zp[(b / BPG) * 16] & 15u);
+                z1 = -static_cast<float>(zp[(b / BPG) * 16 + 8] & 15u);
+              }
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = __int_as_float(part[n][e]) - kMagic;
+                if (ZERO) {
+                  const float d0 = static_cast<float>(begin[n].x), d1 = static_cast<float>(begin[n].y);
+                  v[0] = fmaf(z0, d0, v[0]);
+                  v[1] = fmaf(z0, d1, v[1]);
+                  v[2] = fmaf(z1, d0, v[2]);
+                  v[3] = fmaf(z1, d1, v[3]);
+                }
+                const float u0 = __int_as_float(begin[n].z), u1 = __int_as_float(begin[n].w);
+                acc[n][0] = fmaf(s0f * u0, v[0], acc[n][0]);
+                acc[n][1] = fmaf(s0f * u1, v[1], acc[n][1]);
+                acc[n][2] = fmaf(s1f * u0, v[2], acc[n][2]);
+                acc[n][3] = fmaf(s1f * u1, v[3], acc[n][3]);
+              }
             }
           }
-          if (cs == p.chunk_steps) {
+        };
+#pragma unroll 2
+        for (int u = 0; u < n_steps; ++u) {
+          step(u);
+          ++f;
+          if (++cs == ns) {
+            flush();
+            f += spt - ns;
             cs = 0;
             ++ct;
           }
         }
+        __syncwarp();  // the stage has been read
+        issue();
+        cst = cst + 1 == kDepth ? 0 : cst + 1;
       }
-      cp_async_wait<0>();
+      if (cs > 0) flush();
+    }
+    if (!ok) {  // a copy never came (its time limit has passed): wait for those in flight, then leave
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) mbar_drain(&bars[warp][d], (phase >> d) & 1u);
     }
     __syncthreads();
-    // Sums over the warps that had a part of the tile, in warp order.
-    const int orow = p.gated ? 8 : 16;
-    for (int i = tid; i < nt * orow * nrow; i += kWarps * 32) {
-      const int r = i % orow, rest = i / orow;
-      const int m = rest % nrow, t = rest / nrow;
-      float s = 0.f, s2 = 0.f;
-      for (int w = 0; w < kWarps; ++w) {
-        const int a = total * w / kWarps, b = total * (w + 1) / kWarps;
-        if (a >= b || a >= (t + 1) * p.chunk_steps || b <= t * p.chunk_steps) continue;
-        const float* slot = red + static_cast<size_t>(t + w) * 16 * COLS;
+    // Sums over the warps that had a part of a tile, in their order; then over the digits
+    const int log_rows = p.gated ? 3 : 4, orow = 1 << log_rows;
+    for (int i = tid; i < nt * orow * p.slab_rows; i += kWarps * 32) {
+      const int r = i & (orow - 1), tm = i >> log_rows;
+      const int t = div_by(tm, p.by_rows), m = tm - t * p.slab_rows;
+      if (m >= nrow) continue;
+      const int n = (tb + t) * orow + r;
+      if (n >= (p.gated ? p.N / 2 : p.N)) continue;
+      float s[2][ND];
 #pragma unroll
-        for (int c = 0; c < PARTS; ++c) {
-          s += slot[r * COLS + m * PARTS + c];
-          if (p.gated) s2 += slot[(r + 8) * COLS + m * PARTS + c];
+      for (int d = 0; d < ND; ++d) s[0][d] = s[1][d] = 0.f;
+      // the warps that have the tile's first and last step
+      const int w_lo = static_cast<unsigned>(t * spt) / static_cast<unsigned>(per);
+      const int w_hi = static_cast<unsigned>((t + 1) * spt - 1) / static_cast<unsigned>(per);
+#pragma unroll 4
+      for (int w = w_lo; w <= w_hi; ++w) {
+        const float* slot = red + (t + w) * 16 * COLS + r * COLS + m * ND;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          s[0][d] += slot[d];
+          if (p.gated) s[1][d] += slot[8 * COLS + d];
         }
       }
-      const int n = (tb + t) * orow + r;
-      if (n < (p.gated ? p.N / 2 : p.N)) {
-        if (p.gated) s = s / (1.f + expf(-s)) * s2;
-        static_cast<X*>(p.y)[(row0 + m) * p.ldy + n] = from_f32<X>(s);
+      float out[2] = {0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        out[0] += s[0][d];
+        out[1] += s[1][d];
       }
+      if (row_odd[m]) {
+        for (int h = 0; h <= p.gated; ++h) {
+          for (int k = 0; k < p.K; ++k) {
+            const float xv = to_f32<X>(x[m * p.ldx + k]);
+            if (!finite_bits(xv)) out[h] += w4_at<X>(p, tb + t, r + 8 * h, k) * xv;
+          }
+        }
+      }
+      if (p.gated) out[0] = out[0] / (1.f + expf(-out[0])) * out[1];
+      static_cast<X*>(p.y)[(row0 + m) * p.ldy + n] = from_f32<X>(out[0]);
     }
     __syncthreads();
   }
 }
 
-template <typename T, typename X, int NT, int GPS, bool ZERO>
-int launch_stream(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows,
+template <typename X, int NT, int GPS, bool ZERO>
+int launch_stream(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows, int* status,
                   cudaStream_t st) {
-  constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
+  constexpr int ND = Digits<X>::N;
   constexpr int COLS = 8 * NT;
+  constexpr int ROWS = COLS / ND;
+  constexpr int SIDE = GPS * 16 * static_cast<int>(sizeof(X)) + (ZERO ? GPS * 16 : 0);
+  constexpr int kUnit = unit_of(SIDE);
+  constexpr int STAGE = kUnit * (kStepBytes + SIDE);
   W4Params p;
-  p.codes = static_cast<const unsigned char*>(w->codes);
-  p.scales = static_cast<const unsigned char*>(w->scales);
-  p.zeros = static_cast<const unsigned char*>(w->zeros);
+  p.data = static_cast<const unsigned char*>(w->data);
+  p.zeros = w->zeros;
   p.x = x;
   p.y = y;
   p.ldx = ldx;
   p.ldy = ldy;
+  p.status = status;
   p.rows = rows;
   p.N = w->N;
   p.K = w->K;
   p.gated = w->gated;
   p.g = w4_geom(w);
-  p.stage_bytes = kStepBytes + GPS * 16 * static_cast<int>(sizeof(X)) + (ZERO ? GPS * 16 : 0);
-  const int ccols = std::min(COLS, rows * PARTS);
-  const int slabs = (rows * PARTS + COLS / PARTS * PARTS - 1) / (COLS / PARTS * PARTS);
-  // x of as many steps as fit 96 KB, in chunks of one length
-  const int fit = std::max(1, (96 * 1024 / (ccols * 2) - 32) / 128);
+  p.vec = ldx % (16 / static_cast<int>(sizeof(X))) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const int ccols = std::min(COLS, rows * ND);
+  const int slabs = (rows + ROWS - 1) / ROWS;
+  const int grid = std::min(p.g.tiles, std::max(1, 148 / slabs));
+  p.tpb = std::min(NT > 2 ? 4 : 16, (p.g.tiles + grid - 1) / grid);
+  const int fixed = kWarps * kDepth * STAGE + (p.tpb + kWarps - 1) * 16 * COLS * 4;
+  // x of as many steps as fit, in chunks of one length
+  const int per_step = ccols * 128 + GPS * COLS * 8;
+  const int fit = (kMaxSmem - 2048 - fixed - ccols * 16) / per_step / kUnit * kUnit;
+  if (fit < kUnit) return KATA_ERR_UNSUPPORTED;
   const int chunks = (p.g.steps + fit - 1) / fit;
-  p.chunk_steps = (p.g.steps + chunks - 1) / chunks;
-  const int grid = std::min(p.g.tiles, std::max(1, 148 * 2 / slabs));
-  p.tpb = std::min(8, (p.g.tiles + grid - 1) / grid);
-  const size_t smem = static_cast<size_t>(ccols) * (p.chunk_steps * 128 + 32) * 2 + kWarps * kDepth * p.stage_bytes +
-                      static_cast<size_t>(p.tpb + kWarps - 1) * 16 * COLS * 4;
-  auto kern = w4_stream_kernel<T, X, NT, GPS, ZERO>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e != cudaSuccess) return KATA_ERR_CUDA;
+  p.tiles_q = p.g.tiles / grid;
+  p.tiles_r = p.g.tiles % grid;
+  p.slab_rows = std::min(ROWS, rows);
+  p.wpr = kWarps / p.slab_rows;
+  p.by_rows = recip(p.slab_rows);
+  p.by_wpr = recip(p.wpr);
+  p.chunk_steps = chunks == 1 ? p.g.steps : ((p.g.steps + chunks - 1) / chunks + kUnit - 1) / kUnit * kUnit;
+  p.chunks = (p.g.steps + p.chunk_steps - 1) / p.chunk_steps;
+  p.by_steps = recip(p.chunk_steps);
+  const size_t smem = fixed + static_cast<size_t>(p.chunk_steps) * per_step + ccols * 16;
+  auto kern = w4_stream_kernel<X, NT, GPS, ZERO>;
+  static std::atomic<uint64_t> allowed{0};
+  if (int e = allow_smem(reinterpret_cast<const void*>(kern), kMaxSmem - 2048, allowed)) return e;
   kern<<<dim3(grid, slabs), kWarps * 32, smem, st>>>(p);
   return from_cuda(cudaGetLastError());
 }
 
-template <typename T, typename X, int NT>
+template <typename X, int NT>
 int launch_groups(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows,
-                  cudaStream_t st) {
+                  int* status, cudaStream_t st) {
   const int gps = w->group < 128 ? 128 / w->group : 1;
   if (w->zeros) {
-    if (gps == 4) return launch_stream<T, X, NT, 4, true>(w, x, ldx, y, ldy, rows, st);
-    if (gps == 2) return launch_stream<T, X, NT, 2, true>(w, x, ldx, y, ldy, rows, st);
-    return launch_stream<T, X, NT, 1, true>(w, x, ldx, y, ldy, rows, st);
+    if (gps == 4) return launch_stream<X, NT, 4, true>(w, x, ldx, y, ldy, rows, status, st);
+    if (gps == 2) return launch_stream<X, NT, 2, true>(w, x, ldx, y, ldy, rows, status, st);
+    return launch_stream<X, NT, 1, true>(w, x, ldx, y, ldy, rows, status, st);
   }
-  if (gps == 4) return launch_stream<T, X, NT, 4, false>(w, x, ldx, y, ldy, rows, st);
-  if (gps == 2) return launch_stream<T, X, NT, 2, false>(w, x, ldx, y, ldy, rows, st);
-  return launch_stream<T, X, NT, 1, false>(w, x, ldx, y, ldy, rows, st);
+  if (gps == 4) return launch_stream<X, NT, 4, false>(w, x, ldx, y, ldy, rows, status, st);
+  if (gps == 2) return launch_stream<X, NT, 2, false>(w, x, ldx, y, ldy, rows, status, st);
+  return launch_stream<X, NT, 1, false>(w, x, ldx, y, ldy, rows, status, st);
 }
 
-template <typename T, typename X>
+template <typename X>
 int launch_rows(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows,
-                cudaStream_t st) {
-  const int cols = rows * (sizeof(X) == 4 ? 3 : 1);
-  if (cols <= (sizeof(X) == 4 ? 6 : 8)) return launch_groups<T, X, 1>(w, x, ldx, y, ldy, rows, st);
-  if (cols <= (sizeof(X) == 4 ? 15 : 16)) return launch_groups<T, X, 2>(w, x, ldx, y, ldy, rows, st);
-  return launch_groups<T, X, 4>(w, x, ldx, y, ldy, rows, st);
+                int* status, cudaStream_t st) {
+  const int cols = rows * Digits<X>::N;
+  if (cols <= 8) return launch_groups<X, 1>(w, x, ldx, y, ldy, rows, status, st);
+  if (cols <= 16) return launch_groups<X, 2>(w, x, ldx, y, ldy, rows, status, st);
+  if (cols <= 24) return launch_groups<X, 3>(w, x, ldx, y, ldy, rows, status, st);
+  return launch_groups<X, 4>(w, x, ldx, y, ldy, rows, status, st);
 }
 
 int w4_check(const kata_w4_weight* w) {
@@ -434,7 +568,7 @@ int w4_check(const kata_w4_weight* w) {
   if (w->dtype != KATA_DTYPE_F32 && w->dtype != KATA_DTYPE_BF16 && w->dtype != KATA_DTYPE_F16) return KATA_ERR_DTYPE;
   if (w->N < 1 || w->K < 1 || w->N > (1 << 24) || w->K > (1 << 24)) return KATA_ERR_SHAPE;
   if (w->group != 32 && w->group != 64 && (w->group < 128 || w->group % 128)) return KATA_ERR_SHAPE;
-  if (w->gated != 0 && w->gated != 1) return KATA_ERR_INVALID;
+  if ((w->gated != 0 && w->gated != 1) || (w->zeros != 0 && w->zeros != 1)) return KATA_ERR_INVALID;
   if (w->gated && w->N % 2) return KATA_ERR_SHAPE;
   return KATA_OK;
 }
@@ -447,41 +581,29 @@ bool w4_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0
 
 using namespace kata;
 
-extern "C" int kata_w4_layout(const kata_w4_weight* w, size_t* code_bytes, size_t* scale_bytes, size_t* zero_bytes) {
-  if (int e = w4_check(w)) return e;
+extern "C" size_t kata_w4_bytes(const kata_w4_weight* w) {
+  if (w4_check(w)) return 0;
   const W4Geom g = w4_geom(w);
-  if (code_bytes) *code_bytes = static_cast<size_t>(g.tiles) * g.steps * kStepBytes;
-  if (scale_bytes) *scale_bytes = static_cast<size_t>(g.tiles) * g.groups * 16 * w4_esize(w->dtype);
-  if (zero_bytes) *zero_bytes = static_cast<size_t>(g.tiles) * g.groups * 16;
-  return KATA_OK;
+  return static_cast<size_t>(g.tiles) * g.steps * g.rec;
 }
 
 extern "C" int kata_w4_pack(const void* packed, const void* scales, const void* zeros, const kata_w4_weight* w,
                             kata_stream_t stream) {
   if (int e = w4_check(w)) return e;
-  if (!packed || !scales || !w->codes || !w->scales || (!zeros) != (!w->zeros)) return KATA_ERR_INVALID;
-  if (!w4_al16(w->codes) || !w4_al16(w->scales) || (w->zeros && !w4_al16(w->zeros))) return KATA_ERR_ALIGN;
+  if (!packed || !scales || !w->data || (!zeros) != (!w->zeros)) return KATA_ERR_INVALID;
+  if (!w4_al16(w->data)) return KATA_ERR_ALIGN;
   const W4Geom g = w4_geom(w);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const long long words = static_cast<long long>(g.tiles) * g.steps * (kStepBytes / 4);
-  const long long ns = static_cast<long long>(g.tiles) * g.groups * 16;
-  const int G = (w->K + w->group - 1) / w->group;
-  auto grid = [](long long n) { return static_cast<int>(std::min<long long>(148 * 16, (n + 255) / 256)); };
-  w4_pack_codes_kernel<<<grid(words), 256, 0, st>>>(static_cast<const uint32_t*>(packed),
-                                                    static_cast<uint32_t*>(const_cast<void*>(w->codes)), w->N, w->K,
-                                                    w->gated, g.steps, words);
+  const int grid = static_cast<int>(std::min<long long>(148 * 8, (static_cast<long long>(g.tiles) * g.steps + 7) / 8));
+  const uint32_t* pk = static_cast<const uint32_t*>(packed);
+  const uint8_t* z = static_cast<const uint8_t*>(zeros);
+  unsigned char* data = static_cast<unsigned char*>(const_cast<void*>(w->data));
   if (w->dtype == KATA_DTYPE_F32)
-    w4_pack_scales_kernel<uint32_t><<<grid(ns), 256, 0, st>>>(static_cast<const uint32_t*>(scales),
-                                                              static_cast<uint32_t*>(const_cast<void*>(w->scales)), w->N,
-                                                              G, w->gated, g.groups, ns, 0u);
+    w4_pack_kernel<uint32_t><<<grid, 256, 0, st>>>(pk, static_cast<const uint32_t*>(scales), z, data, w->N, w->K, w->group,
+                                                   w->gated, g);
   else
-    w4_pack_scales_kernel<uint16_t><<<grid(ns), 256, 0, st>>>(static_cast<const uint16_t*>(scales),
-                                                              static_cast<uint16_t*>(const_cast<void*>(w->scales)), w->N,
-                                                              G, w->gated, g.groups, ns, static_cast<uint16_t>(0));
-  if (zeros)
-    w4_pack_scales_kernel<uint8_t><<<grid(ns), 256, 0, st>>>(static_cast<const uint8_t*>(zeros),
-                                                             static_cast<uint8_t*>(const_cast<void*>(w->zeros)), w->N, G,
-                                                             w->gated, g.groups, ns, static_cast<uint8_t>(8));
+    w4_pack_kernel<uint16_t><<<grid, 256, 0, st>>>(pk, static_cast<const uint16_t*>(scales), z, data, w->N, w->K, w->group,
+                                                   w->gated, g);
   return from_cuda(cudaGetLastError());
 }
 
@@ -490,26 +612,25 @@ extern "C" int kata_w4_linear(const kata_w4_weight* w, const void* x, long long 
   if (int e = w4_check(w)) return e;
   if (rows < 0 || rows > (1ll << 30)) return KATA_ERR_SHAPE;
   if (rows == 0) return KATA_OK;
-  if (!w->codes || !w->scales || !x || !y) return KATA_ERR_INVALID;
-  if (!w4_al16(w->codes) || !w4_al16(w->scales) || (w->zeros && !w4_al16(w->zeros))) return KATA_ERR_ALIGN;
+  if (!w->data || !x || !y) return KATA_ERR_INVALID;
+  if (!w4_al16(w->data)) return KATA_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(x) % w4_esize(w->dtype) || reinterpret_cast<uintptr_t>(y) % w4_esize(w->dtype))
     return KATA_ERR_ALIGN;
   if (rows > 1 && (ldx < w->K || ldy < (w->gated ? w->N / 2 : w->N))) return KATA_ERR_SHAPE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int slab = w->dtype == KATA_DTYPE_F32 ? 10 : 32;  // rows per slab of the widest form; slabs are the grid's y
+  const int slab = 8;  // rows per slab of the widest form; slabs are the grid's y
   for (long long r = 0; r < rows; r += 65535ll * slab) {
     const int n = static_cast<int>(std::min<long long>(rows - r, 65535ll * slab));
     const unsigned char* xr = static_cast<const unsigned char*>(x) + r * ldx * w4_esize(w->dtype);
     unsigned char* yr = static_cast<unsigned char*>(y) + r * ldy * w4_esize(w->dtype);
     int e;
     if (w->dtype == KATA_DTYPE_BF16)
-      e = launch_rows<__nv_bfloat16, __nv_bfloat16>(w, xr, ldx, yr, ldy, n, st);
+      e = launch_rows<__nv_bfloat16>(w, xr, ldx, yr, ldy, n, status, st);
     else if (w->dtype == KATA_DTYPE_F16)
-      e = launch_rows<__half, __half>(w, xr, ldx, yr, ldy, n, st);
+      e = launch_rows<__half>(w, xr, ldx, yr, ldy, n, status, st);
     else
-      e = launch_rows<__nv_bfloat16, float>(w, xr, ldx, yr, ldy, n, st);
+      e = launch_rows<float>(w, xr, ldx, yr, ldy, n, status, st);
     if (e) return e;
   }
-  (void)status;
   return KATA_OK;
 }

@@ -13,8 +13,6 @@ counterpart.  Inference only (no autograd).  There is no CPU path.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -54,23 +52,24 @@ class W4Weight:
         self.in_features, self.group_size, self.activation = K, int(group_size), activation
         self.dtype, self.device = scales.dtype, dev
         L = _lib.lib()
-        a = _lib.W4WeightArgs(N=N, K=K, group=int(group_size), dtype=_lib.DTYPE[scales.dtype],
-                              gated=int(activation == "swiglu"))
-        sizes = [ctypes.c_size_t() for _ in range(3)]
-        _lib.check(L.kata_w4_layout(a, *sizes), "kata_w4_layout")
-        with torch.cuda.device(dev):
-            buf = [torch.empty(n.value, dtype=torch.uint8, device=dev) for n in sizes[:2 if zeros is None else 3]]
-            a.codes, a.scales = buf[0].data_ptr(), buf[1].data_ptr()
-            a.zeros = buf[2].data_ptr() if zeros is not None else None
+        a = _lib.W4WeightArgs(None, N, K, int(group_size), _lib.DTYPE[scales.dtype], int(activation == "swiglu"),
+                              int(zeros is not None))
+        n = L.kata_w4_bytes(a)
+        if n == 0:
+            raise ValueError(f"unsupported 4-bit weight: N={N}, K={K}, group_size={group_size} (32, 64 or a multiple of "
+                             f"128), activation={activation!r} (an even N)")
+        with _lib.on_device(dev):
+            data = torch.empty(n, dtype=torch.uint8, device=dev)
+            a.data = data.data_ptr()
             pc, sc, zc = packed.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
             _lib.check(L.kata_w4_pack(pc.data_ptr(), sc.data_ptr(), _lib.ptr(zc), a, _lib.stream_handle(dev)),
                        "kata_w4_pack")
-        self._buffers, self._args = buf, a
+        self._data, self._args = data, a
 
     @property
     def nbytes(self) -> int:
         """Device bytes of the laid-out codes, scales and zero points."""
-        return sum(b.numel() for b in self._buffers)
+        return self._data.numel()
 
 
 def w4_linear(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
@@ -81,19 +80,21 @@ def w4_linear(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
         raise RuntimeError(f"x is on {x.device}, the weight on {w.device}")
     if x.dtype != w.dtype:
         raise TypeError(f"x is {x.dtype}, the weight's scales are {w.dtype}")
-    K = w.in_features
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f"x must be (..., {K}), got {tuple(x.shape)}")
-    if x.dim() != 2 or x.stride(1) != 1 or (x.stride(0) < K and x.shape[0] > 1):
-        x2 = x.reshape(-1, K).contiguous()
-    else:
-        x2 = x
+    K, shape = w.in_features, x.shape
+    if not shape or shape[-1] != K:
+        raise ValueError(f"x must be (..., {K}), got {tuple(shape)}")
+    x2 = x if len(shape) == 2 else x.reshape(-1, K)
+    ldx, one = x2.stride()
     rows = x2.shape[0]
-    y = torch.empty(*x.shape[:-1], w.out_features, dtype=x.dtype, device=x.device)
+    if one != 1 or (ldx < K and rows > 1):
+        x2 = x2.contiguous()
+        ldx = K
+    dev = w.device
+    y = torch.empty(*shape[:-1], w.out_features, dtype=w.dtype, device=dev)
     if rows:
-        with _lib.on_device(x.device):
-            rc = _lib.lib().kata_w4_linear(w._args, x2.data_ptr(), x2.stride(0), y.data_ptr(), w.out_features, rows,
-                                           _lib.status_word(x.device).data_ptr(), _lib.stream_handle(x.device))
+        with _lib.on_device(dev):
+            rc = _lib.lib().kata_w4_linear(w._args, x2.data_ptr(), ldx, y.data_ptr(), w.out_features, rows,
+                                           _lib.status_word(dev).data_ptr(), _lib.stream_handle(dev))
         if rc:
             _lib.check(rc, "kata_w4_linear")
     return y

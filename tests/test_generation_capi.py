@@ -3,8 +3,6 @@ their Python fronts refuse CPU tensors."""
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 
@@ -20,20 +18,15 @@ def L():
 
 
 def w4(**kw):
-    return _lib.W4WeightArgs(**{**dict(codes=16, scales=16, N=32, K=128, group=64, dtype=1, gated=0), **kw})
+    return _lib.W4WeightArgs(**{**dict(data=16, N=32, K=128, group=64, dtype=1, gated=0, zeros=0), **kw})
 
 
-def test_w4_layout_sizes(L):
-    def sizes(**kw):
-        s = [ctypes.c_size_t() for _ in range(3)]
-        assert L.kata_w4_layout(w4(**kw), *s) == 0
-        return [v.value for v in s]
-
-    # tiles of 16 rows, steps of 128 k: 1 KB of codes a step, 16 scales a group
-    assert sizes() == [2 * 1024, 2 * 2 * 16 * 2, 2 * 2 * 16]
-    assert sizes(N=33, K=129, group=32, dtype=0) == [3 * 2 * 1024, 3 * 8 * 16 * 4, 3 * 8 * 16]
-    assert sizes(N=34, K=700, group=256, gated=1) == [3 * 6 * 1024, 3 * 3 * 16 * 2, 3 * 3 * 16]
-    assert L.kata_w4_layout(w4(), None, None, None) == 0
+def test_w4_sizes(L):
+    # tiles of 16 rows (8 pairs of a gated weight), steps of 128 k: 1 KB of codes and 16 scales (zeros) a group
+    assert L.kata_w4_bytes(w4()) == 2 * (1024 + 2 * 16 * 2)
+    assert L.kata_w4_bytes(w4(N=33, K=129, group=32, dtype=0, zeros=1)) == 3 * 2 * (1024 + 4 * 16 * 5)
+    assert L.kata_w4_bytes(w4(N=34, K=700, group=256, gated=1)) == 3 * 6 * (1024 + 16 * 2)
+    assert L.kata_w4_bytes(w4(group=48)) == 0
 
 
 def test_w4_refusals(L):
@@ -44,9 +37,9 @@ def test_w4_refusals(L):
                 dict(N=31, gated=1), dict(N=1 << 25)):
         assert L.kata_w4_linear(w4(**bad), *ok) == -3, bad
     assert L.kata_w4_linear(w4(gated=2), *ok) == -1
-    assert L.kata_w4_linear(w4(codes=None), *ok) == -1
-    assert L.kata_w4_linear(w4(codes=24), *ok) == -4
-    assert L.kata_w4_linear(w4(zeros=24), *ok) == -4
+    assert L.kata_w4_linear(w4(zeros=2), *ok) == -1
+    assert L.kata_w4_linear(w4(data=None), *ok) == -1
+    assert L.kata_w4_linear(w4(data=24), *ok) == -4
     assert L.kata_w4_linear(w4(), None, 128, 16, 32, 1, None, None) == -1
     assert L.kata_w4_linear(w4(), 17, 128, 16, 32, 1, None, None) == -4
     assert L.kata_w4_linear(w4(), 16, 127, 16, 32, 2, None, None) == -3
@@ -55,7 +48,7 @@ def test_w4_refusals(L):
     assert L.kata_w4_linear(w4(), None, 128, None, 32, 0, None, None) == 0  # no rows: nothing to do
     assert L.kata_w4_pack(None, 16, None, w4(), None) == -1
     assert L.kata_w4_pack(16, 16, 16, w4(), None) == -1  # zeros without a place for them
-    assert L.kata_w4_pack(16, 16, None, w4(scales=20), None) == -4
+    assert L.kata_w4_pack(16, 16, None, w4(data=20), None) == -4
 
 
 def test_qkv_step_refusals(L):

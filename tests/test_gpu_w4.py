@@ -184,9 +184,9 @@ def test_w4_refusals():
         W4Weight(packed, scales.double(), z, in_features=128, group_size=64)
     with pytest.raises(ValueError):
         W4Weight(packed, scales, z, in_features=128, group_size=64, activation="gelu")
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         W4Weight(packed, scales[:, :1], None, in_features=128, group_size=160)  # neither 32, 64 nor whole 128s
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         W4Weight(packed[:31], scales[:31], None, in_features=128, group_size=64, activation="swiglu")  # odd rows
     with pytest.raises(RuntimeError):
         W4Weight(packed.cpu(), scales.cpu(), None, in_features=128, group_size=64)
