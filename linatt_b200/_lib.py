@@ -258,7 +258,9 @@ def lib() -> ctypes.CDLL:
             L.kata_w4_pack.restype = c_int
             L.kata_w4_pack.argtypes = [c_void_p, c_void_p, c_void_p, P_W4, c_void_p]
             L.kata_w4_linear.restype = c_int
-            L.kata_w4_linear.argtypes = [P_W4, c_void_p, c_ll, c_void_p, c_ll, c_ll, c_void_p, c_void_p]
+            L.kata_w4_linear.argtypes = [P_W4, c_void_p, c_ll, c_void_p, c_ll, c_ll, c_void_p, c_size_t, c_void_p, c_void_p]
+            L.kata_w4_workspace_bytes.restype = c_size_t
+            L.kata_w4_workspace_bytes.argtypes = [P_W4, c_void_p, c_ll, c_ll]
             L.kata_qkv_step.restype = c_int
             L.kata_qkv_step.argtypes = ([ctypes.POINTER(QkvStepArgs), c_void_p, c_ll] + [c_void_p] * 5 +
                                         [c_ll, c_void_p])

@@ -563,6 +563,491 @@ int launch_rows(const kata_w4_weight* w, const void* x, long long ldx, void* y, 
   return launch_groups<X, 4>(w, x, ldx, y, ldy, rows, status, st);
 }
 
+// ------------------------------------------------------------------------------------------------
+// Tensor-core kernel: more rows than that.
+//
+// The weight is the A operand: 128 of its rows (8 tiles) by a step of 128 k, turned to 16-bit floats by the
+// unpack warps straight into tensor memory (a row is a TMEM lane, so a thread unpacks words of its own
+// row), and x the B operand by TMA: nothing of A passes through shared memory, whose bandwidth B needs.
+// Codes to floats: a code as a byte beside 0x43 (0x64) is 128 + code in bf16 (1024 + code in f16), and one
+// fused multiply-add leaves unit (code - zero), exactly.  With bf16 the unit is 2^-10: a group's sum stays
+// finite for every finite x; the scale takes it back.  fp32 x is three bf16 parts, each a column.
+//
+// A group's products go to one of 2 or 4 accumulators; the drain warps add it, times the rows' scales, to
+// fp32 registers while another one fills, so that scales stay exact.  Unpacking and draining have warps of
+// their own: in one loop each waits for what the other has just started (1750 cycles a step measured).
+// With few row blocks a cluster's CTAs split k and add their sums through shared memory.
+// ------------------------------------------------------------------------------------------------
+
+template <typename T>
+struct Magic;
+template <>
+struct Magic<__nv_bfloat16> {
+  static constexpr uint32_t base = 0x43434343u;
+  static constexpr float back = 1024.f;
+  static __device__ __forceinline__ uint32_t offset(uint32_t zero) {  // -(128 + zero) 2^-10
+    const __nv_bfloat162 v = __float2bfloat162_rn(-(128.f + static_cast<float>(zero)) * (1.f / 1024.f));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b) {
+    const uint32_t u = 0x3a803a80u;  // 2^-10
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&u),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+template <>
+struct Magic<__half> {
+  static constexpr uint32_t base = 0x64646464u;
+  static constexpr float back = 1.f;
+  static __device__ __forceinline__ uint32_t offset(uint32_t zero) { return 0xe400e400u + 0x00010001u * zero; }
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b) {
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+// The eight codes of a word, in order, as four pairs
+template <typename T>
+__device__ __forceinline__ void unpack8(uint32_t word, uint32_t offset, uint32_t* out) {
+  const uint32_t lo = word & 0x0f0f0f0fu, hi = (word >> 4) & 0x0f0f0f0fu;
+  out[0] = Magic<T>::fma2(__byte_perm(lo, Magic<T>::base, 0x4140), offset);
+  out[1] = Magic<T>::fma2(__byte_perm(lo, Magic<T>::base, 0x4342), offset);
+  out[2] = Magic<T>::fma2(__byte_perm(hi, Magic<T>::base, 0x4140), offset);
+  out[3] = Magic<T>::fma2(__byte_perm(hi, Magic<T>::base, 0x4342), offset);
+}
+
+// An fp32 value as three bf16 parts, each the leading 8 bits of what is left: exact together, and no
+// part overflows.  Infinities and NaN stay in the first part.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+  const float a = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  const bool fin = finite_bits(x);
+  const float r = fin ? x - a : 0.f;
+  const float b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+  p[0] = __float2bfloat16_rn(fin ? a : x);
+  p[1] = __float2bfloat16_rn(b);
+  p[2] = __float2bfloat16_rn(r - b);
+}
+
+// x in the form that TMA takes: [part][row][ld], ld a multiple of 8 (fp32 rows as their parts, 16-bit rows that
+// do not lie on 16-byte boundaries as they are)
+template <typename T, typename X>
+__global__ void __launch_bounds__(256) w4_parts_kernel(const X* __restrict__ x, long long ldx, T* __restrict__ out, long long rows,
+                                                       int K, int ld) {
+  const long long n = rows * ld;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const long long r = i / ld;
+    const int k = static_cast<int>(i - r * ld);
+    const X v = k < K ? x[r * ldx + k] : from_f32<X>(0.f);
+    if constexpr (sizeof(X) == 4) {
+      __nv_bfloat16 p[3];
+      split3(v, p);
+#pragma unroll
+      for (int c = 0; c < 3; ++c) out[c * n + i] = p[c];
+    } else {
+      out[i] = v;
+    }
+  }
+}
+
+__device__ __forceinline__ void tma_load_x(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void arrive_warp(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+
+// n MMAs (4 or 2) along k inside one 64-column box of x, one election for all: the MMA warp shares its scheduler
+// with busy warps, and every instruction it does not issue counts
+template <int n>
+__device__ __forceinline__ void umma_ts_chain(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (n == 4)
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "add.u64 b1, %2, 2;\n\tadd.u64 b2, %2, 4;\n\tadd.u64 b3, %2, 6;\n\t"
+        "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 b1;\n\t.reg .b32 a1;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "add.u64 b1, %2, 2;\n\tadd.u32 a1, %1, 8;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+struct GemmParams {
+  const unsigned char* data;
+  void* y;
+  long long ldy;
+  int* status;
+  int rows, N, gated, zeros;
+  W4Geom g;
+  int cs;
+};
+
+// Warps: codes' copies, x's copies, MMAs, (an idle one,) 8 drain, 8 unpack.  A copy costs its warp 115 cycles, so codes come
+// in runs of 4 steps of a tile and x has a warp of its own (one warp, a step at a time: 1430 cycles a step).
+constexpr int kRun = 4;
+constexpr int kCodeStages = 2;
+
+template <int R, int PARTS>
+struct GemmSmem {
+  static constexpr int N = R * PARTS;
+  static constexpr int UW = 8;  // unpack warps (16 slow the MMA warp down, which shares its scheduler: 27.9 against 24.7 us)
+  static constexpr int threads = 32 * (12 + UW);
+  static constexpr int XS = N <= 64 ? 6 : N <= 128 ? 4 : 2;  // stages of x, 128 k each
+  static constexpr int REC = 1024 + 4 * 16 * (PARTS == 3 ? 5 : 3);
+  static constexpr int AS = N <= 128 ? 4 : 2;  // TMEM: stages of A, 64 columns each,
+  static constexpr int DS = N <= 64 ? 4 : 2;   // and accumulators of N columns
+  unsigned char x[XS][2][N * 128];
+  unsigned char codes[kCodeStages][8][kRun * REC];
+  uint64_t c_full[kCodeStages], c_free[kCodeStages], x_full[XS], x_free[XS], a_full[AS], a_free[AS], d_full[DS], d_free[DS];
+  uint32_t tmem;
+  int abort;
+};
+
+template <typename T, typename X, int R>
+__global__ void __launch_bounds__(GemmSmem<R, sizeof(X) == 4 ? 3 : 1>::threads, 1) w4_gemm_kernel(const __grid_constant__ CUtensorMap tmx, const GemmParams p) {
+  constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
+  constexpr int N = R * PARTS;
+  constexpr int HALF = R / 2;  // rows of x a thread sums
+  using S = GemmSmem<R, PARTS>;
+  constexpr int XS = S::XS, AS = S::AS, DS = S::DS, UW = S::UW;
+  static_assert(DS * N + AS * 64 <= 512, "TMEM columns");
+  extern __shared__ unsigned char raw[];
+  S& sm = *reinterpret_cast<S*>(raw + (1024 - (smem_u32(raw) & 1023)) % 1024);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = p.cs > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int tile0 = blockIdx.x / p.cs * 8, ntile = min(8, p.g.tiles - tile0);
+  const int row0 = blockIdx.y * R;
+  const int k_lo = p.g.steps * rank / p.cs, ns = p.g.steps * (rank + 1) / p.cs - k_lo;
+  const int gps = p.g.gps;
+  if (tid == 0) {
+    sm.abort = 0;
+    for (int i = 0; i < kCodeStages; ++i) {
+      mbar_init(&sm.c_full[i], 1);
+      mbar_init(&sm.c_free[i], UW + 8);
+    }
+    for (int i = 0; i < XS; ++i) {
+      mbar_init(&sm.x_full[i], 1);
+      mbar_init(&sm.x_free[i], 1);
+    }
+    for (int i = 0; i < AS; ++i) {
+      mbar_init(&sm.a_full[i], UW);
+      mbar_init(&sm.a_free[i], 1);
+    }
+    for (int i = 0; i < DS; ++i) {
+      mbar_init(&sm.d_full[i], 1);
+      mbar_init(&sm.d_free[i], 8);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&sm.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = sm.tmem, tmem_a = tbase + DS * N;
+  const WaitCtx wc{p.status, &sm.abort};
+  float acc[HALF];
+#pragma unroll
+  for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
+
+  if (warp == 0) {
+    // lane t copies the records of tile t
+    const unsigned char* src = p.data + (static_cast<long long>(tile0 + lane) * p.g.steps + k_lo) * p.g.rec;
+    int n = 0;  // runs copied
+    for (; n * kRun < ns; ++n) {
+      const int c = n % kCodeStages, bytes = min(kRun, ns - n * kRun) * p.g.rec;
+      if (n >= kCodeStages && !mbar_wait_w(&sm.c_free[c], (n / kCodeStages - 1) & 1, wc)) break;
+      if (lane == 0) mbar_arrive_expect_tx(&sm.c_full[c], ntile * bytes);
+      __syncwarp();
+      if (lane < ntile) bulk_load(sm.codes[c][lane], src, bytes, &sm.c_full[c]);
+      src += bytes;
+    }
+    if (sm.abort) {  // copies in flight land before the CTA goes
+      for (int i = max(0, n - kCodeStages); i < n; ++i) mbar_drain(&sm.c_full[i % kCodeStages], (i / kCodeStages) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) tma_prefetch_desc(&tmx);
+    int n = 0;
+    for (; n < ns; ++n) {
+      const int xs = n % XS;
+      if (n >= XS && !mbar_wait_w(&sm.x_free[xs], (n / XS - 1) & 1, wc)) break;
+      if (lane == 0) mbar_arrive_expect_tx(&sm.x_full[xs], 2 * N * 128);
+      __syncwarp();
+      if (lane < 2) tma_load_x(sm.x[xs][lane], &tmx, &sm.x_full[xs], (k_lo + n) * 128 + lane * 64, row0);
+    }
+    if (sm.abort) {
+      for (int i = max(0, n - XS); i < n; ++i) mbar_drain(&sm.x_full[i % XS], (i / XS) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    constexpr uint32_t idesc = umma_idesc_f16(128, N, std::is_same<T, __nv_bfloat16>::value, false, false);
+    int gi = 0, s = 0;  // groups and steps issued
+    const uint64_t bd0 = umma_smem_desc(smem_u32(sm.x[0][0]), 16, 1024, 128);
+    auto issue = [&](auto gps_c) {  // the groups of a step as a constant: the issue path is one thread's
+      constexpr int G = decltype(gps_c)::value;
+      int xs = 0, as = 0, ds = 0;
+      uint32_t xph = 0, aph = 0, dph = 1;  // phases of the barriers waited for
+      for (; s < ns; ++s) {
+        if (!mbar_wait_w(&sm.x_full[xs], xph, wc) || !mbar_wait_w(&sm.a_full[as], aph, wc)) return;
+        tc_fence_after();
+        const uint32_t a = tmem_a + as * 64;
+        const uint64_t bd = bd0 + static_cast<uint64_t>(xs * (2 * N * 128 / 16));
+#pragma unroll
+        for (int g = 0; g < G; ++g, ++gi) {
+          if (gi >= DS) {
+            if (!mbar_wait_w(&sm.d_free[ds], dph, wc)) return;
+            tc_fence_after();
+          }
+          constexpr int CH = G == 4 ? 2 : 4;
+#pragma unroll
+          for (int k = 0; k < 8 / G; k += CH) {
+            const int kk = g * (8 / G) + k;
+            umma_ts_chain<CH>(tbase + ds * N, a + 8 * kk, bd + static_cast<uint64_t>(((kk >> 2) * (N * 128) + (kk & 3) * 32) >> 4),
+                              idesc, k > 0);
+          }
+          umma_commit_w(&sm.d_full[ds]);
+          if (++ds == DS) {
+            ds = 0;
+            dph ^= 1;
+          }
+        }
+        umma_commit_w(&sm.a_free[as]);
+        umma_commit_w(&sm.x_free[xs]);
+        if (++xs == XS) {
+          xs = 0;
+          xph ^= 1;
+        }
+        if (++as == AS) {
+          as = 0;
+          aph ^= 1;
+        }
+      }
+    };
+    if (gps == 1)
+      issue(std::integral_constant<int, 1>());
+    else if (gps == 2)
+      issue(std::integral_constant<int, 2>());
+    else
+      issue(std::integral_constant<int, 4>());
+    if (s < ns && s > 0) mbar_drain(&sm.x_free[(s - 1) % XS], ((s - 1) / XS) & 1);
+  } else if (warp >= 12) {  // unpack: the words of a row's q = NQ h ..
+    constexpr int NQ = 16 / UW;
+    const int quad = warp & 3, h = (warp - 12) >> 2;
+    const int tile = quad * 2 + (lane >> 4), r16 = lane & 15;
+    const uint32_t a_at = tmem_a + (static_cast<uint32_t>(32 * quad) << 16) + h * (4 * NQ);
+    const uint32_t words_at = (r16 >> 3) * 512 + (r16 & 7) * 64 + h * (16 * NQ);
+    const uint32_t zeros_at = kStepBytes + gps * 16 * sizeof(X) + r16;
+    uint4 wq[NQ];
+    uint32_t zo[4];  // of the step's blocks of 32 k
+    auto fetch = [&](int s) {  // the words of step s
+      const int run = s / kRun, c = run % kCodeStages;
+      if (s % kRun == 0 && !mbar_wait_w(&sm.c_full[c], (run / kCodeStages) & 1, wc)) return false;
+      const unsigned char* rec = sm.codes[c][tile] + (s % kRun) * p.g.rec;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) wq[i] = *reinterpret_cast<const uint4*>(rec + words_at + 16 * i);
+      if (p.zeros) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) zo[b] = Magic<T>::offset(rec[zeros_at + (b * gps >> 2) * 16] & 15u);
+      }
+      return true;
+    };
+#pragma unroll
+    for (int b = 0; b < 4; ++b) zo[b] = Magic<T>::offset(8);
+    bool ok = ns > 0 && fetch(0);
+    for (int s = 0; ok && s < ns; ++s) {
+      const int as = s % AS;
+      if (s >= AS && !mbar_wait_w(&sm.a_free[as], (s / AS - 1) & 1, wc)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t v[4 * NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) unpack8<T>(b == 0 ? wq[i].x : b == 1 ? wq[i].y : b == 2 ? wq[i].z : wq[i].w, zo[b], v + 4 * i);
+        if constexpr (NQ == 1)
+          tmem_st4(a_at + as * 64 + b * 16, v);
+        else
+          tmem_st8(a_at + as * 64 + b * 16, v);
+      }
+      if (s % kRun == kRun - 1) arrive_warp(&sm.c_free[s / kRun % kCodeStages]);
+      ok = s + 1 >= ns || fetch(s + 1);  // under the stores
+      tmem_wait_st();
+      tc_fence_before();
+      arrive_warp(&sm.a_full[as]);
+    }
+  } else if (warp >= 4) {  // drain
+    const int quad = warp & 3, h = (warp - 4) >> 2;
+    const int tile = quad * 2 + (lane >> 4), r16 = lane & 15;
+    const uint32_t d_at = tbase + (static_cast<uint32_t>(32 * quad) << 16) + h * HALF;
+    int ds = 0;
+    uint32_t dph = 0;
+    for (int s = 0; s < ns; ++s) {
+      const int run = s / kRun, c = run % kCodeStages;
+      if (s % kRun == 0 && !mbar_wait_w(&sm.c_full[c], (run / kCodeStages) & 1, wc)) break;
+      const X* sc = reinterpret_cast<const X*>(sm.codes[c][tile] + (s % kRun) * p.g.rec + kStepBytes) + r16;
+      float scale[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) scale[i] = i < gps ? to_f32<X>(sc[i * 16]) * Magic<T>::back : 0.f;
+      if (s % kRun == kRun - 1) arrive_warp(&sm.c_free[c]);
+      bool ok = true;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= gps) break;
+        if (!(ok = mbar_wait_w(&sm.d_full[ds], dph, wc))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int pt = 0; pt < PARTS; ++pt) {
+#pragma unroll
+          for (int c0 = 0; c0 < HALF; c0 += 16) {
+            uint32_t v[16];
+            tmem_ld16(d_at + ds * N + pt * R + c0, v);
+            tmem_wait_ld();
+            if (pt == PARTS - 1 && c0 + 16 == HALF) {  // all read
+              tc_fence_before();
+              arrive_warp(&sm.d_free[ds]);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[c0 + j] = fmaf(scale[i], __uint_as_float(v[j]), acc[c0 + j]);
+          }
+        }
+        if (++ds == DS) {
+          ds = 0;
+          dph ^= 1;
+        }
+      }
+      if (!ok) break;
+    }
+  }
+  __syncthreads();
+  const bool good = sm.abort == 0;
+
+  // The sums through shared memory, [row of x][128 rows of the weight] (every copy and product has ended): the
+  // registers' code is unrolled, and what follows would be fetched once for each of them (20000 cycles measured)
+  float* buf = reinterpret_cast<float*>(sm.x);
+  if (warp >= 4 && warp < 12) {
+#pragma unroll
+    for (int j = 0; j < HALF; ++j) buf[(((warp - 4) >> 2) * HALF + j) * 128 + (warp & 3) * 32 + lane] = acc[j];
+  }
+  if (p.cs > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp < 16 && good) {
+    const int wrow = (warp & 3) * 32 + lane, r = wrow & 15, t = tile0 + (wrow >> 4);
+    const int n = p.gated ? t * 8 + r : t * 16 + r;
+    const bool mine = p.gated ? r < 8 && n < p.N / 2 : n < p.N;
+    const int m_hi = min(R * (rank + 1) / p.cs, p.rows - row0);
+#pragma unroll 1
+    for (int m = R * rank / p.cs + (warp >> 2); m < m_hi; m += 4) {
+      float v = buf[m * 128 + wrow];
+      if (p.cs > 1) {  // over the CTAs of the cluster, in their order
+        const uint32_t at = smem_u32(buf + m * 128 + wrow);
+        v = 0.f;
+        for (int c = 0; c < p.cs; ++c) v += ld_cluster(mapa_shared(at, c));
+      }
+      if (p.gated) {  // the up row is eight lanes on
+        const float up = __shfl_down_sync(0xffffffffu, v, 8);
+        v = v / (1.f + expf(-v)) * up;
+      }
+      if (mine) static_cast<X*>(p.y)[(row0 + m) * p.ldy + n] = from_f32<X>(v);
+    }
+  }
+  if (p.cs > 1) cluster_sync();  // nobody reads this CTA's sums any more
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tbase, 512);
+}
+
+// Whether x can be read by TMA as it lies
+bool tma_ready(int dtype, const void* x, long long ldx) {
+  return dtype != KATA_DTYPE_F32 && ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+}
+
+template <typename T, typename X, int R>
+int launch_gemm(const kata_w4_weight* w, const void* x, long long ldx, long long plane, void* y, long long ldy, int rows,
+                int* status, cudaStream_t st) {
+  constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
+  GemmParams p;
+  p.data = static_cast<const unsigned char*>(w->data);
+  p.y = y;
+  p.ldy = ldy;
+  p.status = status;
+  p.rows = rows;
+  p.N = w->N;
+  p.gated = w->gated;
+  p.zeros = w->zeros;
+  p.g = w4_geom(w);
+  const int blocks = (p.g.tiles + 7) / 8, slabs = (rows + R - 1) / R;
+  p.cs = 1;
+  while (p.cs < 8 && blocks * slabs * p.cs * 2 <= 148 && p.g.steps >= 4 * p.cs) p.cs *= 2;
+  CUtensorMap tm;
+  const uint64_t dims[3] = {static_cast<uint64_t>(w->K), static_cast<uint64_t>(rows), PARTS};
+  const uint64_t str[2] = {static_cast<uint64_t>(ldx) * 2, static_cast<uint64_t>(PARTS == 1 ? ldx * rows : plane) * 2};
+  const uint32_t box[3] = {64, R, PARTS};
+  if (int e = encode_tmap_16bit(&tm, x, 3, dims, str, box, 128)) return e;
+  auto kern = w4_gemm_kernel<T, X, R>;
+  static std::atomic<uint64_t> allowed{0};
+  const int smem = static_cast<int>(sizeof(GemmSmem<R, PARTS>)) + 1024;
+  if (int e = allow_smem(reinterpret_cast<const void*>(kern), smem, allowed)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks * p.cs, slabs);
+  cfg.blockDim = dim3(GemmSmem<R, PARTS>::threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = p.cs;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.cs > 1 ? 1 : 0;
+  return from_cuda(cudaLaunchKernelEx(&cfg, kern, tm, p));
+}
+
+// More rows than the streaming kernel takes: x as it lies where TMA can read it, else through the workspace.
+template <typename T, typename X>
+int run_gemm(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows, void* ws,
+             int* status, cudaStream_t st) {
+  long long plane = 0;
+  if (!tma_ready(w->dtype, x, ldx)) {
+    const int ld = (w->K + 7) / 8 * 8;
+    plane = static_cast<long long>(rows) * ld;
+    const int grid = static_cast<int>(std::min<long long>(148 * 8, (plane + 255) / 256));
+    w4_parts_kernel<T, X><<<grid, 256, 0, st>>>(static_cast<const X*>(x), ldx, static_cast<T*>(ws), rows, w->K, ld);
+    x = ws;
+    ldx = ld;
+  }
+  if (rows <= 32) return launch_gemm<T, X, 32>(w, x, ldx, plane, y, ldy, rows, status, st);
+  if (sizeof(X) == 4 || rows <= 64) return launch_gemm<T, X, 64>(w, x, ldx, plane, y, ldy, rows, status, st);
+  if constexpr (sizeof(X) == 2) return launch_gemm<T, X, 128>(w, x, ldx, plane, y, ldy, rows, status, st);
+  return KATA_OK;
+}
+
 int w4_check(const kata_w4_weight* w) {
   if (!w) return KATA_ERR_INVALID;
   if (w->dtype != KATA_DTYPE_F32 && w->dtype != KATA_DTYPE_BF16 && w->dtype != KATA_DTYPE_F16) return KATA_ERR_DTYPE;
@@ -573,6 +1058,14 @@ int w4_check(const kata_w4_weight* w) {
   return KATA_OK;
 }
 
+// Rows that are streamed over.  Up to 16 columns (5 rows, 4 of fp32) the streaming kernel is ahead whatever the
+// size (5 x 8192 x 8192: 20.6 against 23.9 us); up to 32 only while a weight is small and the fixed cost counts
+// (8 x 768 x 768: 5.1 against 9.7 us; 8 x 4096 x 4096: 14.9 against 13.8 us).
+int stream_rows(const kata_w4_weight* w) {
+  const W4Geom g = w4_geom(w);
+  const bool small = static_cast<long long>(g.tiles) * g.steps <= 4096;
+  return w->dtype == KATA_DTYPE_F32 ? (small ? 8 : 4) : (small ? 10 : 5);
+}
 size_t w4_esize(int dtype) { return dtype == KATA_DTYPE_F32 ? 4 : 2; }
 bool w4_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -607,30 +1100,33 @@ extern "C" int kata_w4_pack(const void* packed, const void* scales, const void* 
   return from_cuda(cudaGetLastError());
 }
 
+extern "C" size_t kata_w4_workspace_bytes(const kata_w4_weight* w, const void* x, long long ldx, long long rows) {
+  if (w4_check(w) || rows <= stream_rows(w) || tma_ready(w->dtype, x, ldx)) return 0;
+  return static_cast<size_t>(rows) * ((w->K + 7) / 8 * 8) * (w->dtype == KATA_DTYPE_F32 ? 6 : 2);
+}
+
 extern "C" int kata_w4_linear(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy,
-                              long long rows, int* status, kata_stream_t stream) {
+                              long long rows, void* workspace, size_t workspace_bytes, int* status,
+                              kata_stream_t stream) {
   if (int e = w4_check(w)) return e;
-  if (rows < 0 || rows > (1ll << 30)) return KATA_ERR_SHAPE;
+  if (rows < 0 || rows > (1ll << 21)) return KATA_ERR_SHAPE;  // slabs of at least 32 rows are the grid's y
   if (rows == 0) return KATA_OK;
   if (!w->data || !x || !y) return KATA_ERR_INVALID;
   if (!w4_al16(w->data)) return KATA_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(x) % w4_esize(w->dtype) || reinterpret_cast<uintptr_t>(y) % w4_esize(w->dtype))
     return KATA_ERR_ALIGN;
   if (rows > 1 && (ldx < w->K || ldy < (w->gated ? w->N / 2 : w->N))) return KATA_ERR_SHAPE;
+  const size_t need = kata_w4_workspace_bytes(w, x, ldx, rows);
+  if (need && (!workspace || workspace_bytes < need)) return KATA_ERR_WORKSPACE;
+  if (need && !w4_al16(workspace)) return KATA_ERR_ALIGN;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int slab = 8;  // rows per slab of the widest form; slabs are the grid's y
-  for (long long r = 0; r < rows; r += 65535ll * slab) {
-    const int n = static_cast<int>(std::min<long long>(rows - r, 65535ll * slab));
-    const unsigned char* xr = static_cast<const unsigned char*>(x) + r * ldx * w4_esize(w->dtype);
-    unsigned char* yr = static_cast<unsigned char*>(y) + r * ldy * w4_esize(w->dtype);
-    int e;
-    if (w->dtype == KATA_DTYPE_BF16)
-      e = launch_rows<__nv_bfloat16>(w, xr, ldx, yr, ldy, n, status, st);
-    else if (w->dtype == KATA_DTYPE_F16)
-      e = launch_rows<__half>(w, xr, ldx, yr, ldy, n, status, st);
-    else
-      e = launch_rows<float>(w, xr, ldx, yr, ldy, n, status, st);
-    if (e) return e;
+  const int n = static_cast<int>(rows);
+  if (rows <= stream_rows(w)) {
+    if (w->dtype == KATA_DTYPE_BF16) return launch_rows<__nv_bfloat16>(w, x, ldx, y, ldy, n, status, st);
+    if (w->dtype == KATA_DTYPE_F16) return launch_rows<__half>(w, x, ldx, y, ldy, n, status, st);
+    return launch_rows<float>(w, x, ldx, y, ldy, n, status, st);
   }
-  return KATA_OK;
+  if (w->dtype == KATA_DTYPE_BF16) return run_gemm<__nv_bfloat16, __nv_bfloat16>(w, x, ldx, y, ldy, n, workspace, status, st);
+  if (w->dtype == KATA_DTYPE_F16) return run_gemm<__half, __half>(w, x, ldx, y, ldy, n, workspace, status, st);
+  return run_gemm<__nv_bfloat16, float>(w, x, ldx, y, ldy, n, workspace, status, st);
 }

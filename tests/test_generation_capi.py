@@ -30,7 +30,7 @@ def test_w4_sizes(L):
 
 
 def test_w4_refusals(L):
-    ok = (16, 128, 16, 32, 1, None, None)
+    ok = (16, 128, 16, 32, 1, None, 0, None, None)
     assert L.kata_w4_linear(None, *ok) == -1
     assert L.kata_w4_linear(w4(dtype=3), *ok) == -2
     for bad in (dict(group=0), dict(group=16), dict(group=96), dict(group=130), dict(N=0), dict(K=0),
@@ -40,12 +40,18 @@ def test_w4_refusals(L):
     assert L.kata_w4_linear(w4(zeros=2), *ok) == -1
     assert L.kata_w4_linear(w4(data=None), *ok) == -1
     assert L.kata_w4_linear(w4(data=24), *ok) == -4
-    assert L.kata_w4_linear(w4(), None, 128, 16, 32, 1, None, None) == -1
-    assert L.kata_w4_linear(w4(), 17, 128, 16, 32, 1, None, None) == -4
-    assert L.kata_w4_linear(w4(), 16, 127, 16, 32, 2, None, None) == -3
-    assert L.kata_w4_linear(w4(), 16, 128, 16, 31, 2, None, None) == -3
-    assert L.kata_w4_linear(w4(), 16, 128, 16, 32, -1, None, None) == -3
-    assert L.kata_w4_linear(w4(), None, 128, None, 32, 0, None, None) == 0  # no rows: nothing to do
+    assert L.kata_w4_linear(w4(), None, 128, 16, 32, 1, None, 0, None, None) == -1
+    assert L.kata_w4_linear(w4(), 17, 128, 16, 32, 1, None, 0, None, None) == -4
+    assert L.kata_w4_linear(w4(), 16, 127, 16, 32, 2, None, 0, None, None) == -3
+    assert L.kata_w4_linear(w4(), 16, 128, 16, 31, 2, None, 0, None, None) == -3
+    assert L.kata_w4_linear(w4(), 16, 128, 16, 32, -1, None, 0, None, None) == -3
+    assert L.kata_w4_linear(w4(), None, 128, None, 32, 0, None, 0, None, None) == 0  # no rows: nothing to do
+    # many rows off 16-byte boundaries, or fp32 ones, are laid out in a workspace
+    assert L.kata_w4_workspace_bytes(w4(), 16, 128, 100) == 0 and L.kata_w4_workspace_bytes(w4(), 18, 128, 1) == 0
+    assert L.kata_w4_workspace_bytes(w4(K=100), 18, 100, 100) == 100 * 104 * 2
+    assert L.kata_w4_workspace_bytes(w4(dtype=0), 16, 128, 100) == 100 * 128 * 6
+    assert L.kata_w4_linear(w4(), 18, 128, 16, 32, 100, None, 0, None, None) == -5
+    assert L.kata_w4_linear(w4(), 18, 128, 16, 32, 100, 8, 25600, None, None) == -4
     assert L.kata_w4_pack(None, 16, None, w4(), None) == -1
     assert L.kata_w4_pack(16, 16, 16, w4(), None) == -1  # zeros without a place for them
     assert L.kata_w4_pack(16, 16, None, w4(data=20), None) == -4
