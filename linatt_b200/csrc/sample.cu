@@ -10,15 +10,22 @@
 // The token is the first in vocabulary order whose inclusive mass, over the kept tokens, exceeds u Z.
 //
 // A filter's cut is the element of the order where the inclusive count reaches k (or the inclusive mass
-// p Z_k).  It is found by digits: a histogram over 2048 bins of the distance from the maximum, then over
-// the bits of the logit and of the index within the bin that holds the cut, until at most kList elements
-// are left, which are sorted.  After the first histogram that is nearly always so; when the whole
-// beginning of the order up to top-k fits the list, everything after it happens on the list.
+// p Z_k).
+//   top-k: a histogram of counts over 2048 bins of the distance from the maximum gives the cut's bin; when
+//   the beginning of the order up to that bin fits a list of kList elements, it is gathered and sorted, and
+//   everything after it happens on the list.
+//   top-p: a pass sums the masses and counts bins of the exponent, 1/128 wide; the counts times the bins'
+//   middles say nearly where the cut is.  A second pass sums what lies before the bins around it, which the
+//   draw needs anyway, and gathers those bins: whether the cut is among them is then known exactly, and if so
+//   the sorted list has it.  (Exact masses in a histogram cost two atomics a token, one with its result.)
+//   Where a list overflows (thousands of nearly equal logits at the cut) or misses, the cut is found by
+//   digits instead: histograms of the distance, then of the bits of the logit and of the index, each within
+//   the bin of the one before.
 //
 // One pass over HBM: a cluster of up to 8 CTAs shares a row (fewer with more rows), each keeping its part
-// in shared memory where it fits (else it is read again, from L2).  Histograms are merged, and the list
-// is gathered in the first CTA, through distributed shared memory.  A call of one row is bound by the
-// latency of these steps, a large batch by the instructions of the histogram's exponentials.
+// in shared memory where it fits (else it is read again, from L2).  Histograms are merged, and lists and sums
+// gathered in the first CTA, through distributed shared memory.  A call of one row is bound by the latency
+// of these steps, a large batch by the instructions of its passes, the exponentials first.
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
@@ -35,6 +42,8 @@ constexpr int kST = 512;  // threads per CTA
 constexpr int kSW = kST / 32;
 constexpr int kBins = 2048;
 constexpr int kList = 2048;          // elements sorted directly
+constexpr int kFine = 2 * kBins;     // bins of the exponent
+constexpr int kChunks = 8 * kSW;     // warps of a row
 constexpr int kTile = 256;           // elements a warp takes at once: 8 a lane
 constexpr int kStage = 96 * 1024;    // bytes of a part of a row that are kept in shared memory
 typedef unsigned long long u64;
@@ -70,32 +79,48 @@ __device__ __forceinline__ u64 order_of(float x, int i) { return static_cast<u64
 
 struct Row {
   float m, inv;  // maximum, 1 / temperature
-  __device__ __forceinline__ float z(float x) const { return x == m ? 0.f : __fmul_rn(__fsub_rn(x, m), inv); }
-  // a mask weighs nothing even at an infinite temperature, nor does anything beside an infinite logit
+  bool odd;      // an infinite maximum or temperature
+  // A mask weighs nothing even at an infinite temperature, nor does anything beside an infinite logit.  Otherwise
+  // exp gives both by itself.
+  __device__ __forceinline__ float z(float x) const { return odd && x == m ? 0.f : __fmul_rn(__fsub_rn(x, m), inv); }
   __device__ __forceinline__ float w(float x) const {
-    return x == m ? 1.f : (x == -INFINITY || m == INFINITY) ? 0.f : expf(z(x));
+    if (odd) return x == m ? 1.f : (x == -INFINITY || m == INFINITY) ? 0.f : expf(z(x));
+    return expf(z(x));
   }
-  __device__ __forceinline__ int bin(float x) const {
-    return x == m ? 0 : static_cast<int>(fminf(__fmul_rn(__fsub_rn(m, x), 64.f), static_cast<float>(kBins - 1)));
+  // Whole numbers growing with the distance from the maximum: adding 2^23 rounds to one and leaves it in the low bits
+  __device__ __forceinline__ static uint32_t whole(float t, int last) {
+    return __float_as_uint(__fadd_rn(fminf(t, static_cast<float>(last)), 8388608.f)) - 0x4b000000u;
+  }
+  __device__ __forceinline__ uint32_t bin(float x) const {
+    return odd && x == m ? 0u : whole(__fmul_rn(__fsub_rn(m, x), 64.f), kBins - 1);
+  }
+  __device__ __forceinline__ uint32_t fine(float x, float z) const {  // an infinitely distant mask's 0 * inf is not a number
+    return odd && !(z <= 0.f) ? kFine - 1u : whole(__fmul_rn(z, -128.f), kFine - 1);
   }
 };
 // rint(w 2^40) for w in [0, 1], in two parts of 20 bits: adding 1.5 2^23 rounds to a whole number and leaves it
 // in the low bits (the conversion to 64 bits runs at a sixteenth of the rate)
-__device__ __forceinline__ u64 mass_of(float w) {
+__device__ __forceinline__ void mass_parts(float w, int& hi, int& lo) {
   const float magic = 12582912.f;
   const float t = w * 1048576.f, h = __fadd_rn(t, magic);
-  const float l = __fadd_rn(__fmul_rn(__fsub_rn(t, __fsub_rn(h, magic)), 1048576.f), magic);
-  return static_cast<u64>((static_cast<long long>(__float_as_int(h) - 0x4b400000) << 20) + (__float_as_int(l) - 0x4b400000));
+  const float l = __fmaf_rn(__fsub_rn(t, __fsub_rn(h, magic)), 1048576.f, magic);
+  hi = __float_as_int(h) - 0x4b400000;
+  lo = __float_as_int(l) - 0x4b400000;
+}
+__device__ __forceinline__ u64 mass_of(float w) {
+  int hi, lo;
+  mass_parts(w, hi, lo);
+  return static_cast<u64>((static_cast<long long>(hi) << 20) + lo);
 }
 
 struct alignas(16) Smem {  // the part of the row follows it, in 16-byte vectors
-  uint32_t cnt[kBins];           // histogram of counts, or the low words of the masses'
-  uint32_t hi[kBins];            // and their high words
+  uint32_t cnt[kFine];           // a histogram of counts; of masses, low words and from kBins on the high ones
   u64 list[kList];               // first CTA
+  u64 keep[kChunks], sure[kChunks];  // first CTA: of each warp of the row, what it keeps and what lies before the cut
   u64 wsum[kSW], scan[kSW];
-  u64 part;                      // what this CTA tells the others
-  u64 before, cut;
-  uint32_t n_list, bin, n_bin;
+  u64 part, part2;               // what this CTA tells the others
+  u64 before, cut, total;
+  uint32_t n_list, bin, bin_hi, n_bin;
 };
 
 __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
@@ -153,41 +178,65 @@ struct Sampler {
     else
       __syncthreads();
   }
-  // The eight logits from place e (a multiple of 8); -inf outside the row and for NaN
-  __device__ __forceinline__ void load(int e, float (&v)[8]) const {
+  // The eight logits from place e (a multiple of 8) as they lie; -inf outside the row
+  struct alignas(16) Eight {
+    T t[8];
+    __device__ __forceinline__ float operator[](int j) const { return fmaxf(to_f32<T>(t[j]), -INFINITY); }  // NaN: -inf
+  };
+  __device__ __forceinline__ Eight load(int e) const {
+    Eight r;
     const T* src = x + (e - skew);
     if (e >= skew && e + 8 <= skew + p.V) {
-      alignas(16) T t[8];
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-        reinterpret_cast<uint4*>(t)[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(t[j]);
+        reinterpret_cast<uint4*>(r.t)[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = e + j >= skew && e + j < skew + p.V ? to_f32<T>(src[j]) : -INFINITY;
+      for (int j = 0; j < 8; ++j) r.t[j] = e + j >= skew && e + j < skew + p.V ? src[j] : from_f32<T>(-INFINITY);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (v[j] != v[j]) v[j] = -INFINITY;
+    return r;
   }
-  __device__ __forceinline__ void get(int e, float (&v)[8]) const {
-    if (!p.staged) return load(e, v);
-    alignas(16) T t[8];
+  __device__ __forceinline__ Eight get(int e) const {
+    if (!p.staged) return load(e);
+    Eight r;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(stage + (e - lo))[i];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(t[j]);
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(r.t)[i] = reinterpret_cast<const uint4*>(stage + (e - lo))[i];
+    return r;
   }
-  // f(logit, index) over the places [a, b) a lane at a time, for a warp; whole tiles
+  __device__ __forceinline__ static float max8(const Eight& r) {
+    float m;
+    if constexpr (sizeof(T) == 4) {
+      m = r[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) m = fmaxf(m, r[j]);
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2* q = reinterpret_cast<const T2*>(r.t);
+      const T2 a = __hmax2(__hmax2(q[0], q[1]), __hmax2(q[2], q[3]));  // a number where there is one
+      m = fmaxf(fmaxf(to_f32<T>(a.x), to_f32<T>(a.y)), -INFINITY);
+    }
+    return m;
+  }
+  // f(eight logits, place) over the places [a, b), for a warp; whole tiles
   template <typename F>
-  __device__ __forceinline__ void each(int a, int b, F f) const {
+  __device__ __forceinline__ void each8(int a, int b, F f) const {
+    if (a >= b) return;
+    Eight next = get(a + lane * 8);
     for (int e = a + lane * 8; e < b; e += kTile) {
-      float v[8];
-      get(e, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f(v[j], e + j - skew);
+      const Eight r = next;
+      if (e + kTile < b) next = get(e + kTile);  // on its way while this one is worked on
+      f(r, e);
     }
+  }
+  // f(logit, index) over those with a logit of at least `floor` among their eight
+  template <typename F>
+  __device__ __forceinline__ void each(int a, int b, float floor, F f) const {
+    each8(a, b, [&](const Eight& r, int e) {
+      if (__any_sync(0xffffffffu, max8(r) >= floor)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f(r[j], e + j - skew);
+      }
+    });
   }
   __device__ __forceinline__ int warp_lo() const { return lo + warp * (p.seg / kSW); }
   __device__ __forceinline__ int warp_hi() const { return min(warp_lo() + p.seg / kSW, (skew + p.V + kTile - 1) / kTile * kTile); }
@@ -208,9 +257,10 @@ struct Sampler {
     return base + inc - mine;
   }
 
-  // The bin of the whole row's histogram where the inclusive sum reaches rem: s.bin, s.before, s.n_bin everywhere
+  // The bin of the whole row's histogram where the inclusive sum reaches rem: s.bin, s.before, s.n_bin everywhere;
+  // false when it does not
   template <bool BY_MASS>
-  __device__ void find_bin(u64 rem) {
+  __device__ bool find_bin(u64 rem) {
     sync();  // histograms are complete
     const int per = kBins / p.cs, first = rank * per;  // this CTA's bins; 4 a thread at most
     u64 v[4] = {0, 0, 0, 0}, sum = 0;
@@ -221,10 +271,10 @@ struct Sampler {
         u64 t = 0;
         for (int c = 0; c < p.cs; ++c) {
           if (p.cs == 1) {
-            t = s.cnt[b0 + j] + (BY_MASS ? static_cast<u64>(s.hi[b0 + j]) << 32 : 0);
+            t = s.cnt[b0 + j] + (BY_MASS ? static_cast<u64>(s.cnt[kBins + b0 + j]) << 32 : 0);
           } else {
             t += ld32_cluster(remote(&s.cnt[b0 + j], c));
-            if (BY_MASS) t += static_cast<u64>(ld32_cluster(remote(&s.hi[b0 + j], c))) << 32;
+            if (BY_MASS) t += static_cast<u64>(ld32_cluster(remote(&s.cnt[kBins + b0 + j], c))) << 32;
           }
         }
         v[j] = t;
@@ -236,7 +286,12 @@ struct Sampler {
     if (p.cs > 1) {
       if (tid == 0) s.part = total;
       cluster_sync();
-      for (int c = 0; c < rank; ++c) before += ld64_cluster(remote(&s.part, c));
+      total = 0;
+      for (int c = 0; c < p.cs; ++c) {
+        const u64 t = ld64_cluster(remote(&s.part, c));
+        if (c < rank) before += t;
+        total += t;
+      }
     }
     for (int j = 0; j < mine; ++j) {
       if (before < rem && before + v[j] >= rem) {
@@ -249,6 +304,64 @@ struct Sampler {
       before += v[j];
     }
     sync();
+    return total >= rem;
+  }
+
+  // The first and last bin of the exponent that may well hold the element where the mass reaches rem: s.bin, s.bin_hi
+  // everywhere.  A bin's mass is taken as its count times its middle's, give or take a thousandth.
+  __device__ void find_range(u64 rem) {
+    sync();  // histograms are complete
+    const int per = kFine / p.cs, mine = per / kST;  // 1 to 8 bins a thread
+    const int b0 = rank * per + tid * mine;
+    u64 low = 0, high = 0;
+    uint32_t n[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      n[j] = 0;
+      if (j < mine) {
+        if (p.cs == 1)
+          n[j] = s.cnt[b0 + j];
+        else
+          for (int c = 0; c < p.cs; ++c) n[j] += ld32_cluster(remote(&s.cnt[b0 + j], c));
+        high += n[j] * most(b0 + j);
+        low += n[j] * least(b0 + j);
+      }
+    }
+    u64 all_low, all_high;
+    low = block_before(low, &all_low);
+    high = block_before(high, &all_high);
+    if (tid == 0) s.bin = s.bin_hi = kFine - 1;
+    if (p.cs > 1) {
+      if (tid == 0) {
+        s.part = all_low;
+        s.part2 = all_high;
+      }
+      cluster_sync();
+      for (int c = 0; c < rank; ++c) {
+        low += ld64_cluster(remote(&s.part, c));
+        high += ld64_cluster(remote(&s.part2, c));
+      }
+    } else {
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j >= mine) break;
+      const u64 dl = n[j] * least(b0 + j), dh = n[j] * most(b0 + j);
+      for (int c = 0; c < p.cs; ++c) {
+        if (high < rem && high + dh >= rem) st32_cluster(remote(&s.bin, c), b0 + j);
+        if (low < rem && low + dl >= rem) st32_cluster(remote(&s.bin_hi, c), b0 + j);
+      }
+      low += dl;
+      high += dh;
+    }
+    sync();
+  }
+  __device__ __forceinline__ static u64 most(int b) {
+    return static_cast<u64>(exp2f(b * (-1.44269504f / 128)) * (1.001f * 1099511627776.f)) + 1;
+  }
+  __device__ __forceinline__ static u64 least(int b) {
+    return b == kFine - 1 ? 0 : static_cast<u64>(exp2f(b * (-1.44269504f / 128)) * (0.999f * 1099511627776.f));
   }
 
   // Ascending sort of the first n of the list (the first CTA alone)
@@ -274,21 +387,41 @@ struct Sampler {
     __syncthreads();
   }
 
-  // Appends to the first CTA's list what `want` chooses
-  template <typename F>
-  __device__ void gather(F want) {
-    each(warp_lo(), warp_hi(), [&](float v, int i) {
-      const bool yes = v > -INFINITY && want(v, i);
-      const unsigned m = __ballot_sync(0xffffffffu, yes);
-      if (m) {
-        const int leader = __ffs(m) - 1;
-        uint32_t at = 0;
-        if (lane == leader) at = add32_cluster(remote(&s.n_list, 0), __popc(m));
-        at = __shfl_sync(0xffffffffu, at, leader) + __popc(m & ((1u << lane) - 1));
-        if (yes && at < kList) st64_cluster(remote(&s.list[at], 0), order_of(v, i));
-      }
-    });
-    sync();
+  // Appends to the first CTA's list (the whole warp)
+  __device__ __forceinline__ void append(bool yes, float v, int i) {
+    const unsigned m = __ballot_sync(0xffffffffu, yes);
+    if (m) {
+      const int leader = __ffs(m) - 1;
+      uint32_t at = 0;
+      if (lane == leader) at = add32_cluster(remote(&s.n_list, 0), __popc(m));
+      at = __shfl_sync(0xffffffffu, at, leader) + __popc(m & ((1u << lane) - 1));
+      if (yes && at < kList) st64_cluster(remote(&s.list[at], 0), order_of(v, i));
+    }
+  }
+  // A logit that every one of the first `b` bins of the distance is above
+  __device__ __forceinline__ float floor_of(uint32_t b) const {
+    return row.odd || b >= kBins - 1 ? -INFINITY : __fsub_rn(row.m, (b + 2) * (1.f / 64)) - fabsf(row.m) * 1e-6f;
+  }
+
+  // Sorts the list (first CTA) and finds where its inclusive sum reaches rem: s.cut; false when it does not
+  template <bool BY_MASS>
+  __device__ bool cut_in_list(int n, u64 rem) {
+    sort_list(n);
+    u64 q[4], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid * 4 + j;
+      q[j] = i >= n ? 0 : BY_MASS ? mass_of(row.w(key_value(static_cast<uint32_t>(s.list[i] >> 32)))) : 1;
+      sum += q[j];
+    }
+    u64 b = block_before(sum, &total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (b < rem && b + q[j] >= rem) s.cut = s.list[tid * 4 + j];
+      b += q[j];
+    }
+    __syncthreads();
+    return total >= rem;
   }
 
   // Finds the first token of the order whose inclusive count (BY_MASS: inclusive mass) is at least `limit`,
@@ -302,10 +435,10 @@ struct Sampler {
       // digits in turn: distance bin, key bits (11, 11, 10), index bits (11, 11)
       const int shift = level == 1 ? 53 : level == 2 ? 42 : level == 3 ? 32 : level == 4 ? 11 : 0;
       const uint32_t width = level == 3 ? 1023u : 2047u;
-      for (int i = tid; i < kBins; i += kST) s.cnt[i] = s.hi[i] = 0;
+      for (int i = tid; i < kBins; i += kST) s.cnt[i] = s.cnt[kBins + i] = 0;
       if (tid == 0) s.n_list = 0;
       __syncthreads();
-      each(warp_lo(), warp_hi(), [&](float v, int i) {
+      each(warp_lo(), warp_hi(), b1 < 0 ? -INFINITY : floor_of(b1), [&](float v, int i) {
         if (v == -INFINITY) return;
         uint32_t d = row.bin(v);
         if (level > 0) {
@@ -318,12 +451,17 @@ struct Sampler {
           if (q == 0) return;
           const uint32_t ql = static_cast<uint32_t>(q), old = atomicAdd(&s.cnt[d], ql);
           const uint32_t qh = static_cast<uint32_t>(q >> 32) + (old + ql < old ? 1u : 0u);
-          if (qh) atomicAdd(&s.hi[d], qh);
+          if (qh) atomicAdd(&s.cnt[kBins + d], qh);
         } else {
           atomicAdd(&s.cnt[d], 1u);
         }
       });
-      find_bin<BY_MASS>(rem);
+      // masked tokens end the order and have no mass: with fewer than k others nothing is cut
+      if (!find_bin<BY_MASS>(rem)) {
+        s.cut = ~0ull;
+        __syncthreads();
+        return false;
+      }
       const uint32_t d = s.bin;
       const u64 before = s.before;
       const uint32_t n_bin = s.n_bin;
@@ -331,7 +469,9 @@ struct Sampler {
       if (level == 0) {
         b1 = d;
         if (!BY_MASS && before + n_bin <= kList) {
-          gather([&](float v, int) { return row.bin(v) <= b1; });
+          each(warp_lo(), warp_hi(), floor_of(b1),
+               [&](float v, int i) { append(v > -INFINITY && row.bin(v) <= static_cast<uint32_t>(b1), v, i); });
+          sync();
           if (rank == 0) sort_list(s.n_list);
           return true;
         }
@@ -340,25 +480,13 @@ struct Sampler {
         mask |= static_cast<u64>(width) << shift;
       }
       if (BY_MASS || n_bin <= kList) {
-        gather([&](float v, int i) { return row.bin(v) == b1 && ((order_of(v, i) ^ prefix) & mask) == 0; });
+        each(warp_lo(), warp_hi(), floor_of(b1), [&](float v, int i) {
+          append(v > -INFINITY && static_cast<int>(row.bin(v)) == b1 && ((order_of(v, i) ^ prefix) & mask) == 0, v, i);
+        });
+        sync();
         const uint32_t n = ld32_cluster(remote(&s.n_list, 0));
         if (n <= kList) {
-          if (rank == 0) {
-            sort_list(n);
-            u64 q[4], sum = 0, total;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int i = tid * 4 + j;
-              q[j] = i >= static_cast<int>(n) ? 0 : BY_MASS ? mass_of(row.w(key_value(static_cast<uint32_t>(s.list[i] >> 32)))) : 1;
-              sum += q[j];
-            }
-            u64 b = block_before(sum, &total);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (b < rem && b + q[j] >= rem) s.cut = s.list[tid * 4 + j];
-              b += q[j];
-            }
-          }
+          if (rank == 0) cut_in_list<BY_MASS>(n, rem);
           sync();
           const u64 cut = p.cs > 1 ? ld64_cluster(remote(&s.cut, 0)) : s.cut;
           sync();
@@ -391,59 +519,44 @@ struct Sampler {
 
     // The first token of the order; the row's part into shared memory
     u64 first = ~0ull;
-    uint32_t live = 0;  // logits above -inf
-    for (int e = warp_lo() + lane * 8; e < warp_hi(); e += kTile) {
-      float v[8];
-      load(e, v);
-      if (p.staged) {
-        alignas(16) T t[8];
+    float best = -INFINITY;
+    constexpr int AHEAD = 4;  // loads in flight: the pass over HBM
+    const int hi_e = warp_hi();
+    for (int e0 = warp_lo() + lane * 8; e0 < hi_e; e0 += AHEAD * kTile) {
+      Eight r[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = from_f32<T>(v[j]);
+      for (int u = 0; u < AHEAD; ++u)
+        if (e0 + u * kTile < hi_e) r[u] = load(e0 + u * kTile);
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(stage + (e - lo))[i] = reinterpret_cast<const uint4*>(t)[i];
-      }
-      float m = v[0];
+      for (int u = 0; u < AHEAD; ++u) {
+        const int e = e0 + u * kTile;
+        if (e >= hi_e) break;
+        if (p.staged) {
 #pragma unroll
-      for (int j = 1; j < 8; ++j) m = fmaxf(m, v[j]);
+          for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(stage + (e - lo))[i] = reinterpret_cast<const uint4*>(r[u].t)[i];
+        }
+        const float m = max8(r[u]);
+        if (m > best) {
+          best = m;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) live += v[j] > -INFINITY;
-      if (order_key(m) < static_cast<uint32_t>(first >> 32)) {
-#pragma unroll
-        for (int j = 7; j >= 0; --j)
-          if (v[j] == m) first = order_of(m, e + j - skew);
+          for (int j = 7; j >= 0; --j)
+            if (r[u][j] == m) first = order_of(m, e + j - skew);
+        }
       }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-    live = __reduce_add_sync(0xffffffffu, live);
-    if (lane == 0) {
-      s.wsum[warp] = first;
-      s.scan[warp] = live;
-    }
+    if (lane == 0) s.wsum[warp] = first;
     __syncthreads();
-    live = 0;
 #pragma unroll
-    for (int w = 0; w < kSW; ++w) {
-      first = min(first, s.wsum[w]);
-      live += static_cast<uint32_t>(s.scan[w]);
-    }
+    for (int w = 0; w < kSW; ++w) first = min(first, s.wsum[w]);
     if (p.cs > 1) {
-      if (tid == 0) {
-        s.part = first;
-        s.n_bin = live;
-      }
+      if (tid == 0) s.part = first;
       cluster_sync();
-      live = 0;
-      for (int c = 0; c < p.cs; ++c) {
-        first = min(first, ld64_cluster(remote(&s.part, c)));
-        live += ld32_cluster(remote(&s.n_bin, c));
-      }
+      for (int c = 0; c < p.cs; ++c) first = min(first, ld64_cluster(remote(&s.part, c)));
       cluster_sync();
     }
-    const float m = key_value(static_cast<uint32_t>(first >> 32));
-    row.m = m;
-    row.inv = temp > 0.f ? 1.f / temp : 1.f;
-    if (first == ~0ull || m == -INFINITY) {  // nothing to draw from
+    if (first == ~0ull) {  // nothing to draw from
       if (rank == 0 && tid == 0) {
         p.token[b] = -1;
         p.logprob[b] = -INFINITY;
@@ -454,10 +567,12 @@ struct Sampler {
       if (rank == 0 && tid == 0) answer(b, static_cast<int>(first & 0xffffffffu), 0, true);
       return;
     }
+    row.m = key_value(static_cast<uint32_t>(first >> 32));
+    row.inv = 1.f / temp;
+    row.odd = row.m == INFINITY || row.inv == 0.f || row.inv == INFINITY;
 
     u64 cut = ~0ull;
-    // masked tokens end the order and have no mass: with no more than k others nothing is cut
-    if (static_cast<uint32_t>(k) < live) {
+    if (k < p.V) {
       if (find_cut<false>(k)) {
         if (rank == 0) from_list(b, k, top_p, p24, min_p, u24);
         sync();
@@ -465,84 +580,191 @@ struct Sampler {
       }
       cut = s.cut;
     }
-    auto kept = [&](float v, int i, bool floor) -> u64 {
-      if (v == -INFINITY || order_of(v, i) > cut) return 0;
-      const float w = row.w(v);
-      return floor && w < min_p ? 0 : mass_of(w);
-    };
     if (top_p < 1.f) {
+      // all masses, and the counts of the exponent's bins
+      for (int i = tid; i < kBins; i += kST) s.cnt[i] = s.cnt[kBins + i] = 0;
+      if (tid == 0) s.n_list = 0;
+      __syncthreads();
       u64 t = 0;
-      each(warp_lo(), warp_hi(), [&](float v, int i) { t += kept(v, i, false); });
+      const float cut_v = key_value(static_cast<uint32_t>(cut >> 32));  // all ones: not a number, above nothing
+      each8(warp_lo(), warp_hi(), [&](const Eight& r, int e) {
+        int hi = 0, lo8 = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = r[j];
+          if (v < cut_v || (v == cut_v && order_of(v, e + j - skew) > cut)) continue;
+          if (row.odd && v == -INFINITY) continue;
+          const float z = row.z(v);
+          int h, l;
+          mass_parts(row.odd ? row.w(v) : expf(z), h, l);
+          hi += h;
+          lo8 += l;
+          if (h | l) atomicAdd(&s.cnt[row.fine(v, z)], 1u);
+        }
+        t += static_cast<u64>((static_cast<long long>(hi) << 20) + lo8);
+      });
       const u64 limit = share(total_of(t), p24, true);
+      find_range(limit);
+      const uint32_t b_lo = s.bin, b_hi = s.bin_hi;
+      // what lies surely before the cut, and a list of what may be the cut
+      const float floor = row.odd || b_hi >= kFine - 1 ? -INFINITY
+                                                       : __fsub_rn(row.m, (b_hi + 2) * (1.f / 128) / row.inv) - fabsf(row.m) * 1e-6f;
+      u64 sure = 0, keep = 0;
+      each(warp_lo(), warp_hi(), floor, [&](float v, int i) {
+        const float z = row.z(v);
+        const uint32_t d = row.fine(v, z);
+        const bool in = !(v < cut_v || (v == cut_v && order_of(v, i) > cut)) && v > -INFINITY;
+        if (in && d < b_lo) {
+          const float w = row.w(v);
+          const u64 q = mass_of(w);
+          sure += q;
+          keep += w < min_p ? 0 : q;
+        }
+        append(in && d >= b_lo && d <= b_hi, v, i);
+      });
+      tell(keep, sure);
+      const uint32_t n = ld32_cluster(remote(&s.n_list, 0));
+      if (n <= kList) {
+        if (rank == 0) {
+          u64 before = 0;
+          for (int c = 0; c < p.cs * kSW; ++c) before += s.sure[c];
+          const bool found = before < limit && cut_in_list<true>(n, limit - before);
+          if (tid == 0) s.n_bin = found;
+          for (int i = tid; found && i < static_cast<int>(n); i += kST) {
+            const u64 o = s.list[i];
+            const float w = row.w(key_value(static_cast<uint32_t>(o >> 32)));
+            if (o <= s.cut && w >= min_p) atomicAdd(&s.keep[(static_cast<uint32_t>(o) + skew) / (p.seg / kSW)], mass_of(w));
+          }
+          __syncthreads();
+        }
+        if (draw(b, u24, min_p, true)) return;
+      }
+      sync();  // everybody has read the list's length
       find_cut<true>(limit);
       cut = min(cut, s.cut);
     }
-    u64 t = 0;
-    each(warp_lo(), warp_hi(), [&](float v, int i) { t += kept(v, i, true); });
-    u64 cta;
-    const u64 total = total_of(t, &cta);
-    const u64 target = share(total, u24, false);
-    u64 base = 0;
-    for (int c = 0; c < rank; ++c) base += ld64_cluster(remote(&s.part, c));
-    if (base <= target && target < base + cta) {  // the token is in this CTA's part: in which warp's?
-      int w = 0;
-      while (target >= base + s.wsum[w]) base += s.wsum[w++];
-      const int a = lo + w * (p.seg / kSW), per = (p.seg / kSW / kTile + kSW - 1) / kSW * kTile;
-      const int end = min(a + p.seg / kSW, (skew + p.V + kTile - 1) / kTile * kTile);
-      const int sa = min(end, a + warp * per), sb = min(end, sa + per);
-      u64 q = 0;
-      each(sa, sb, [&](float v, int i) { q += kept(v, i, true); });
+    u64 keep = 0;
+    if (cut == ~0ull && !row.odd) {
+      each8(warp_lo(), warp_hi(), [&](const Eight& r, int) {
+        int hi = 0, lo8 = 0;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-      if (lane == 0) s.scan[warp] = q;
-      __syncthreads();
-      for (int i = 0; i < warp; ++i) base += s.scan[i];
-      if (base <= target && target < base + q) {
-        for (int e = sa; e < sb; e += kTile) {
-          float v[8];
-          get(e + lane * 8, v);
-          u64 ms[8], sum = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) sum += ms[j] = kept(v[j], e + lane * 8 + j - skew, true);
-          u64 at = base + warp_scan(sum, lane);
-          const unsigned hit = __ballot_sync(0xffffffffu, at > target);
-          base = __shfl_sync(0xffffffffu, at, 31);
-          if (hit) {
-            if (lane == __ffs(hit) - 1) {
-              at -= sum;
-              for (int j = 0; j < 8; ++j) {
-                at += ms[j];
-                if (at > target) {
-                  answer(b, e + lane * 8 + j - skew, total, false);
-                  break;
-                }
-              }
-            }
-            break;
-          }
+        for (int j = 0; j < 8; ++j) {
+          const float w = expf(row.z(r[j]));
+          int h, l;
+          mass_parts(w < min_p ? 0.f : w, h, l);
+          hi += h;
+          lo8 += l;
         }
-      }
+        keep += static_cast<u64>((static_cast<long long>(hi) << 20) + lo8);
+      });
+    } else {
+      each(warp_lo(), warp_hi(), -INFINITY, [&](float v, int i) { keep += kept(v, i, cut, min_p); });
     }
-    sync();  // nobody reads this CTA's sums any more
+    if (rank == 0 && tid == 0) s.cut = cut;
+    tell(keep, 0);
+    draw(b, u24, min_p, false);
   }
 
-  // The row's total of what the threads have, and the CTA's (s.wsum of its warps, s.part for the others)
-  __device__ u64 total_of(u64 mine, u64* cta = nullptr) {
+  __device__ __forceinline__ u64 kept(float v, int i, u64 cut, float min_p) const {
+    if (v == -INFINITY || order_of(v, i) > cut) return 0;
+    const float w = row.w(v);
+    return w < min_p ? 0 : mass_of(w);
+  }
+
+  // A warp's sums to the first CTA
+  __device__ void tell(u64 keep, u64 sure) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      keep += __shfl_xor_sync(0xffffffffu, keep, o);
+      sure += __shfl_xor_sync(0xffffffffu, sure, o);
+    }
+    if (lane == 0) {
+      st64_cluster(remote(&s.keep[rank * kSW + warp], 0), keep);
+      st64_cluster(remote(&s.sure[rank * kSW + warp], 0), sure);
+    }
+    sync();
+  }
+
+  // The token, from the first CTA's s.keep and s.cut; false (`check`) when s.n_bin says that there is no cut yet
+  __device__ bool draw(long long b, u64 u24, float min_p, bool check) {
+    if (rank == 0 && warp == 0) {
+      const int n = p.cs * kSW, per = (n + 31) / 32;  // 1 to 4 chunks a lane
+      u64 sum = 0;
+      for (int j = 0; j < per; ++j) sum += lane * per + j < n ? s.keep[lane * per + j] : 0;
+      u64 at = warp_scan(sum, lane);
+      const u64 total = __shfl_sync(0xffffffffu, at, 31), target = share(total, u24, false);
+      at -= sum;
+      for (int j = 0; j < per; ++j) {
+        const u64 q = lane * per + j < n ? s.keep[lane * per + j] : 0;
+        if (at <= target && target < at + q) {
+          s.bin = lane * per + j;
+          s.before = at;
+          s.part2 = target;
+          s.total = total;
+        }
+        at += q;
+      }
+    }
+    sync();
+    if (check && ld32_cluster(remote(&s.n_bin, 0)) == 0) return false;
+    const int chunk = ld32_cluster(remote(&s.bin, 0));
+    u64 base = ld64_cluster(remote(&s.before, 0));
+    const u64 target = ld64_cluster(remote(&s.part2, 0)), total = ld64_cluster(remote(&s.total, 0));
+    const u64 cut = ld64_cluster(remote(&s.cut, 0));
+    sync();  // nobody reads another CTA's memory any more
+    if (chunk / kSW != rank) return true;
+    // in this CTA's part: its warps split the chunk
+    const int a = lo + chunk % kSW * (p.seg / kSW), per = (p.seg / kSW / kTile + kSW - 1) / kSW * kTile;
+    const int end = min(a + p.seg / kSW, (skew + p.V + kTile - 1) / kTile * kTile);
+    const int sa = min(end, a + warp * per), sb = min(end, sa + per);
+    u64 q = 0;
+    each(sa, sb, -INFINITY, [&](float v, int i) { q += kept(v, i, cut, min_p); });
+#pragma unroll
+    for (int o = 16; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    if (lane == 0) s.scan[warp] = q;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) base += s.scan[i];
+    if (!(base <= target && target < base + q)) return true;
+    for (int e = sa; e < sb; e += kTile) {
+      const Eight r = get(e + lane * 8);
+      u64 ms[8], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += ms[j] = kept(r[j], e + lane * 8 + j - skew, cut, min_p);
+      u64 at = base + warp_scan(sum, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, at > target);
+      base = __shfl_sync(0xffffffffu, at, 31);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) {
+          at -= sum;
+          for (int j = 0; j < 8; ++j) {
+            at += ms[j];
+            if (at > target) {
+              answer(b, e + lane * 8 + j - skew, total, false);
+              break;
+            }
+          }
+        }
+        return true;
+      }
+    }
+    return true;
+  }
+
+  // The row's total of what the threads have
+  __device__ u64 total_of(u64 mine) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    __syncthreads();
     if (lane == 0) s.wsum[warp] = mine;
     __syncthreads();
     u64 all = 0;
 #pragma unroll
     for (int w = 0; w < kSW; ++w) all += s.wsum[w];
-    if (cta) *cta = all;
     if (p.cs == 1) return all;
     if (tid == 0) s.part = all;
     cluster_sync();
     all = 0;
     for (int c = 0; c < p.cs; ++c) all += ld64_cluster(remote(&s.part, c));
-    if (!cta) cluster_sync();  // with `cta` the parts are read again
+    cluster_sync();
     return all;
   }
 
@@ -608,7 +830,7 @@ __global__ void __launch_bounds__(kST) sample_kernel(const SampleParams p) {
   const int rank = p.cs > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int tid = threadIdx.x;
-  Sampler<T> me{p, s, reinterpret_cast<T*>(raw + sizeof(Smem)), x, rank, tid, tid & 31, tid >> 5, skew, rank * p.seg, Row{0.f, 0.f}};
+  Sampler<T> me{p, s, reinterpret_cast<T*>(raw + sizeof(Smem)), x, rank, tid, tid & 31, tid >> 5, skew, rank * p.seg, Row{0.f, 0.f, false}};
   me.run(b);
 }
 
