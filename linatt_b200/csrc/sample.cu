@@ -11,15 +11,16 @@
 //
 // A filter's cut is the element of the order where the inclusive count reaches k (or the inclusive mass
 // p Z_k).
-//   top-k: a histogram of counts over 2048 bins of the distance from the maximum gives the cut's bin; when
-//   the beginning of the order up to that bin fits a list of kList elements, it is gathered and sorted, and
-//   everything after it happens on the list.
-//   top-p: a pass sums the masses and counts bins of the exponent, 1/128 wide; the counts times the bins'
-//   middles say nearly where the cut is.  A second pass sums what lies before the bins around it, which the
+//   top-k: the k-th largest of the threads' maxima (four each) is not above the k-th largest logit; a histogram of the
+//   maxima (four atomics a thread, not one an element) finds it to a bin of 1/64.  When what is at least that
+//   large fits a list of kList elements, it is gathered and sorted, and everything after it happens on the list.
+//   top-p: a pass sums all masses to Z.  What weighs less than (1 - p) Z / V is after the cut whatever the rest
+//   is; the others are counted by bins of the exponent, 1/128 wide (the atomics of a full histogram took three
+//   quarters of a large batch's time), and counts times the bins' middles say nearly where the cut is.  A second pass sums what lies before the bins around it, which the
 //   draw needs anyway, and gathers those bins: whether the cut is among them is then known exactly, and if so
 //   the sorted list has it.  (Exact masses in a histogram cost two atomics a token, one with its result.)
-//   Where a list overflows (thousands of nearly equal logits at the cut) or misses, the cut is found by
-//   digits instead: histograms of the distance, then of the bits of the logit and of the index, each within
+//   Where a list overflows (thousands of equal logits at the cut, as 16-bit types have) or misses, the cut is
+//   found by digits instead: histograms of the distance, then of the bits of the logit and of the index, each within
 //   the bin of the one before.
 //
 // One pass over HBM: a cluster of up to 8 CTAs shares a row (fewer with more rows), each keeping its part
@@ -28,7 +29,6 @@
 // of these steps, a large batch by the instructions of its passes, the exponentials first.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "attn_common.cuh"
 #include "host_util.h"
@@ -132,14 +132,16 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
   return v;
 }
 __device__ __forceinline__ uint32_t remote(const void* p, int rank) { return mapa_shared(smem_u32(p), rank); }
+// Without a memory clobber, so that several are in flight at once (one takes 600 cycles); the barriers around
+// them are volatile too and keep their places.
 __device__ __forceinline__ uint32_t ld32_cluster(uint32_t addr) {
   uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ u64 ld64_cluster(uint32_t addr) {
   u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ void st32_cluster(uint32_t addr, uint32_t v) {
@@ -148,16 +150,50 @@ __device__ __forceinline__ void st32_cluster(uint32_t addr, uint32_t v) {
 __device__ __forceinline__ void st64_cluster(uint32_t addr, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
-__device__ __forceinline__ uint32_t add32_cluster(uint32_t addr, uint32_t v) {
-  uint32_t old;
-  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
-  return old;
-}
-
 // total * n24 / 2^24, rounded down or up
 __device__ __forceinline__ u64 share(u64 total, u64 n24, bool up) {
   const u64 hi = __umul64hi(total, n24), lo = total * n24;
   return (hi << 40) + (lo >> 24) + ((up && (lo & 0xffffffull)) ? 1 : 0);
+}
+
+// Ascending sort of n different numbers by the CTA.  Up to one a thread: each finds its rank (8 cycles a number);
+// beyond that by merging (66 steps of 300 cycles for 2048).
+__device__ __noinline__ void sort_list(u64* list, int n) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (n <= kST) {
+    const u64 mine = tid < n ? list[tid] : 0;
+    int rank = 0;
+    if (tid < (n + 31) / 32 * 32) {
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) rank += list[j] < mine;
+    }
+    __syncthreads();
+    if (tid < n) list[rank] = mine;
+    __syncthreads();
+    return;
+  }
+  int size = 1024;
+  while (size < n) size *= 2;
+  for (int i = n + tid; i < size; i += kST) list[i] = ~0ull;
+  for (int k = 2; k <= size; k *= 2) {
+    for (int j = k / 2; j > 0; j /= 2) {
+      // within 64 numbers a warp's pairs are its own
+      if (j >= 32 || k <= 2)
+        __syncthreads();
+      else
+        __syncwarp();
+      for (int i = tid; i < size / 2; i += kST) {
+        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+        const u64 va = list[a], vb = list[b];
+        if ((va > vb) == ((a & k) == 0)) {
+          list[a] = vb;
+          list[b] = va;
+        }
+      }
+    }
+  }
+  __syncthreads();
 }
 
 template <typename T>
@@ -171,6 +207,13 @@ struct Sampler {
   int lo;          // this CTA's first place
   Row row;
 
+  // A word of each CTA of the row (0 past them), lane by lane
+  __device__ __forceinline__ u64 of_all(const u64* w) const { return lane < p.cs ? ld64_cluster(remote(w, lane)) : 0; }
+  __device__ __forceinline__ static u64 sum32(u64 v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
   __device__ __forceinline__ void sync() const {
     __syncwarp();  // the cluster barrier is one instruction for a warp
     if (p.cs > 1)
@@ -183,18 +226,23 @@ struct Sampler {
     T t[8];
     __device__ __forceinline__ float operator[](int j) const { return fmaxf(to_f32<T>(t[j]), -INFINITY); }  // NaN: -inf
   };
-  __device__ __forceinline__ Eight load(int e) const {
+  __device__ __forceinline__ Eight load_edge(int e) const {
     Eight r;
-    const T* src = x + (e - skew);
-    if (e >= skew && e + 8 <= skew + p.V) {
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-        reinterpret_cast<uint4*>(r.t)[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) r.t[j] = e + j >= skew && e + j < skew + p.V ? src[j] : from_f32<T>(-INFINITY);
-    }
+    for (int j = 0; j < 8; ++j) r.t[j] = e + j >= skew && e + j < skew + p.V ? x[e + j - skew] : from_f32<T>(-INFINITY);
     return r;
+  }
+  __device__ __forceinline__ Eight load(int e) const {
+    if (e < skew || e + 8 > skew + p.V) return load_edge(e);
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+      reinterpret_cast<uint4*>(r.t)[i] = __ldg(reinterpret_cast<const uint4*>(x + (e - skew)) + i);
+    return r;
+  }
+  __device__ __forceinline__ float one(int e) const {  // the logit of a place
+    if (p.staged) return fmaxf(to_f32<T>(stage[e - lo]), -INFINITY);
+    return e >= skew && e < skew + p.V ? fmaxf(to_f32<T>(x[e - skew]), -INFINITY) : -INFINITY;
   }
   __device__ __forceinline__ Eight get(int e) const {
     if (!p.staged) return load(e);
@@ -260,7 +308,7 @@ struct Sampler {
   // The bin of the whole row's histogram where the inclusive sum reaches rem: s.bin, s.before, s.n_bin everywhere;
   // false when it does not
   template <bool BY_MASS>
-  __device__ bool find_bin(u64 rem) {
+  __device__ __forceinline__ bool find_bin(u64 rem) {
     sync();  // histograms are complete
     const int per = kBins / p.cs, first = rank * per;  // this CTA's bins; 4 a thread at most
     u64 v[4] = {0, 0, 0, 0}, sum = 0;
@@ -269,13 +317,17 @@ struct Sampler {
     if (tid * mine < per) {
       for (int j = 0; j < mine; ++j) {
         u64 t = 0;
-        for (int c = 0; c < p.cs; ++c) {
-          if (p.cs == 1) {
-            t = s.cnt[b0 + j] + (BY_MASS ? static_cast<u64>(s.cnt[kBins + b0 + j]) << 32 : 0);
-          } else {
-            t += ld32_cluster(remote(&s.cnt[b0 + j], c));
-            if (BY_MASS) t += static_cast<u64>(ld32_cluster(remote(&s.cnt[kBins + b0 + j], c))) << 32;
+        if (p.cs == 1) {
+          t = s.cnt[b0 + j] + (BY_MASS ? static_cast<u64>(s.cnt[kBins + b0 + j]) << 32 : 0);
+        } else {
+          uint32_t l[8], h[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            l[c] = c < p.cs ? ld32_cluster(remote(&s.cnt[b0 + j], c)) : 0;
+            h[c] = BY_MASS && c < p.cs ? ld32_cluster(remote(&s.cnt[kBins + b0 + j], c)) : 0;
           }
+#pragma unroll
+          for (int c = 0; c < 8; ++c) t += l[c] + (static_cast<u64>(h[c]) << 32);
         }
         v[j] = t;
         sum += t;
@@ -286,12 +338,9 @@ struct Sampler {
     if (p.cs > 1) {
       if (tid == 0) s.part = total;
       cluster_sync();
-      total = 0;
-      for (int c = 0; c < p.cs; ++c) {
-        const u64 t = ld64_cluster(remote(&s.part, c));
-        if (c < rank) before += t;
-        total += t;
-      }
+      const u64 t = of_all(&s.part);
+      before += sum32(lane < rank ? t : 0);
+      total = sum32(t);
     }
     for (int j = 0; j < mine; ++j) {
       if (before < rem && before + v[j] >= rem) {
@@ -309,7 +358,7 @@ struct Sampler {
 
   // The first and last bin of the exponent that may well hold the element where the mass reaches rem: s.bin, s.bin_hi
   // everywhere.  A bin's mass is taken as its count times its middle's, give or take a thousandth.
-  __device__ void find_range(u64 rem) {
+  __device__ __forceinline__ void find_range(u64 rem) {
     sync();  // histograms are complete
     const int per = kFine / p.cs, mine = per / kST;  // 1 to 8 bins a thread
     const int b0 = rank * per + tid * mine;
@@ -319,10 +368,15 @@ struct Sampler {
     for (int j = 0; j < 8; ++j) {
       n[j] = 0;
       if (j < mine) {
-        if (p.cs == 1)
+        if (p.cs == 1) {
           n[j] = s.cnt[b0 + j];
-        else
-          for (int c = 0; c < p.cs; ++c) n[j] += ld32_cluster(remote(&s.cnt[b0 + j], c));
+        } else {
+          uint32_t t[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) t[c] = c < p.cs ? ld32_cluster(remote(&s.cnt[b0 + j], c)) : 0;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) n[j] += t[c];
+        }
         high += n[j] * most(b0 + j);
         low += n[j] * least(b0 + j);
       }
@@ -337,10 +391,9 @@ struct Sampler {
         s.part2 = all_high;
       }
       cluster_sync();
-      for (int c = 0; c < rank; ++c) {
-        low += ld64_cluster(remote(&s.part, c));
-        high += ld64_cluster(remote(&s.part2, c));
-      }
+      const u64 l = of_all(&s.part), h = of_all(&s.part2);
+      low += sum32(lane < rank ? l : 0);
+      high += sum32(lane < rank ? h : 0);
     } else {
       __syncthreads();
     }
@@ -348,10 +401,10 @@ struct Sampler {
     for (int j = 0; j < 8; ++j) {
       if (j >= mine) break;
       const u64 dl = n[j] * least(b0 + j), dh = n[j] * most(b0 + j);
-      for (int c = 0; c < p.cs; ++c) {
-        if (high < rem && high + dh >= rem) st32_cluster(remote(&s.bin, c), b0 + j);
-        if (low < rem && low + dl >= rem) st32_cluster(remote(&s.bin_hi, c), b0 + j);
-      }
+      if (high < rem && high + dh >= rem)
+        for (int c = 0; c < p.cs; ++c) st32_cluster(remote(&s.bin, c), b0 + j);
+      if (low < rem && low + dl >= rem)
+        for (int c = 0; c < p.cs; ++c) st32_cluster(remote(&s.bin_hi, c), b0 + j);
       low += dl;
       high += dh;
     }
@@ -364,39 +417,22 @@ struct Sampler {
     return b == kFine - 1 ? 0 : static_cast<u64>(exp2f(b * (-1.44269504f / 128)) * (0.999f * 1099511627776.f));
   }
 
-  // Ascending sort of the first n of the list (the first CTA alone)
-  __device__ void sort_list(int n) {
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kST) s.list[i] = ~0ull;
-    for (int k = 2; k <= size; k *= 2) {
-      for (int j = k / 2; j > 0; j /= 2) {
-        // within 64 elements a warp's pairs are its own
-        if (j >= 32 || (j == 16 && k == 32) || k <= 2) __syncthreads();
-        else __syncwarp();
-        for (int i = tid; i < size / 2; i += kST) {
-          const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
-          const u64 va = s.list[a], vb = s.list[b];
-          if ((va > vb) == ((a & k) == 0)) {
-            s.list[a] = vb;
-            s.list[b] = va;
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-
-  // Appends to the first CTA's list (the whole warp)
+  // Appends to this CTA's list
   __device__ __forceinline__ void append(bool yes, float v, int i) {
-    const unsigned m = __ballot_sync(0xffffffffu, yes);
-    if (m) {
-      const int leader = __ffs(m) - 1;
-      uint32_t at = 0;
-      if (lane == leader) at = add32_cluster(remote(&s.n_list, 0), __popc(m));
-      at = __shfl_sync(0xffffffffu, at, leader) + __popc(m & ((1u << lane) - 1));
-      if (yes && at < kList) st64_cluster(remote(&s.list[at], 0), order_of(v, i));
-    }
+    if (!yes || *static_cast<volatile uint32_t*>(&s.n_list) > kList) return;  // too many: no more of them queue up
+    const uint32_t at = atomicAdd(&s.n_list, 1u);
+    if (at < kList) s.list[at] = order_of(v, i);
+  }
+  // The CTAs' lists (complete, and a barrier since) to the first one's; returns how many there are: more than kList
+  // are not collected
+  __device__ __forceinline__ uint32_t collect() {
+    if (p.cs == 1) return s.n_list;
+    const uint32_t mine = s.n_list, n = lane < p.cs ? ld32_cluster(remote(&s.n_list, lane)) : 0;
+    const uint32_t all = __reduce_add_sync(0xffffffffu, n), before = __reduce_add_sync(0xffffffffu, lane < rank ? n : 0);
+    if (all <= kList && rank > 0)
+      for (uint32_t i = tid; i < mine; i += kST) st64_cluster(remote(&s.list[before + i], 0), s.list[i]);
+    sync();
+    return all;
   }
   // A logit that every one of the first `b` bins of the distance is above
   __device__ __forceinline__ float floor_of(uint32_t b) const {
@@ -405,8 +441,8 @@ struct Sampler {
 
   // Sorts the list (first CTA) and finds where its inclusive sum reaches rem: s.cut; false when it does not
   template <bool BY_MASS>
-  __device__ bool cut_in_list(int n, u64 rem) {
-    sort_list(n);
+  __device__ __forceinline__ bool cut_in_list(int n, u64 rem) {
+    sort_list(s.list, n);
     u64 q[4], sum = 0, total;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -422,6 +458,26 @@ struct Sampler {
     }
     __syncthreads();
     return total >= rem;
+  }
+
+  // The beginning of the order, the first k at least, as the first CTA's sorted list, by way of the threads' maxima;
+  // false when these are too few or the list overflows
+  __device__ __forceinline__ bool list_top(int k, const float (&tops)[4]) {
+    if (k > p.cs * kST * 2) return false;
+    for (int i = tid; i < kBins; i += kST) s.cnt[i] = 0;
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (tops[j] > -INFINITY) atomicAdd(&s.cnt[row.bin(tops[j])], 1u);
+    if (!find_bin<false>(k)) return false;
+    const uint32_t b1 = s.bin;
+    each(warp_lo(), warp_hi(), floor_of(b1), [&](float v, int i) { append(v > -INFINITY && row.bin(v) <= b1, v, i); });
+    sync();
+    const uint32_t n = collect();
+    if (n <= kList && rank == 0) sort_list(s.list, n);
+    sync();  // everybody has read the list's length
+    return n <= kList;
   }
 
   // Finds the first token of the order whose inclusive count (BY_MASS: inclusive mass) is at least `limit`,
@@ -472,7 +528,8 @@ struct Sampler {
           each(warp_lo(), warp_hi(), floor_of(b1),
                [&](float v, int i) { append(v > -INFINITY && row.bin(v) <= static_cast<uint32_t>(b1), v, i); });
           sync();
-          if (rank == 0) sort_list(s.n_list);
+          const uint32_t n_all = collect();
+          if (rank == 0) sort_list(s.list, n_all);
           return true;
         }
       } else {
@@ -484,7 +541,7 @@ struct Sampler {
           append(v > -INFINITY && static_cast<int>(row.bin(v)) == b1 && ((order_of(v, i) ^ prefix) & mask) == 0, v, i);
         });
         sync();
-        const uint32_t n = ld32_cluster(remote(&s.n_list, 0));
+        const uint32_t n = collect();
         if (n <= kList) {
           if (rank == 0) cut_in_list<BY_MASS>(n, rem);
           sync();
@@ -496,6 +553,60 @@ struct Sampler {
         }
       }
       sync();  // everybody has read the list's length
+    }
+  }
+
+  // The cut by mass among the elements in the exponent's bins b_lo..b_hi (logits of `floor` at least), by the digits of
+  // their keys, counted from the range's first one, and where equal logits are too many, of their indexes: s.cut
+  // everywhere; false when their mass does not reach rem
+  __device__ __forceinline__ bool cut_in_range(u64 rem, uint32_t b_lo, uint32_t b_hi, float floor) {
+    // a logit above all of the range: the slack of `above` the other way
+    const float ceil = row.odd || b_lo < 3 ? INFINITY : __fsub_rn(row.m, (b_lo - 2) * (1.f / 128) / row.inv) + fabsf(row.m) * 1e-6f;
+    uint32_t key = order_key(ceil), span = order_key(floor) - key;  // keys key .. key + span
+    int group = -1;                                                 // of 2048 indexes
+    uint32_t* count = reinterpret_cast<uint32_t*>(s.list);
+    for (;;) {
+      const int shift = max(0, 21 - __clz(span));  // span >> shift < 2048
+      const bool by_index = span == 0;
+      auto in = [&](float v, int i) {
+        const uint32_t d = row.fine(v, row.z(v));
+        return v >= floor && v > -INFINITY && d >= b_lo && d <= b_hi && order_key(v) - key <= span && (group < 0 || i >> 11 == group);
+      };
+      for (int i = tid; i < kBins; i += kST) s.cnt[i] = s.cnt[kBins + i] = count[i] = 0;
+      __syncthreads();
+      each(warp_lo(), warp_hi(), floor, [&](float v, int i) {
+        if (!in(v, i)) return;
+        const uint32_t d = by_index ? i >> 11 : (order_key(v) - key) >> shift;
+        const u64 q = mass_of(row.w(v));
+        const uint32_t ql = static_cast<uint32_t>(q), old = atomicAdd(&s.cnt[d], ql);
+        const uint32_t qh = static_cast<uint32_t>(q >> 32) + (old + ql < old ? 1u : 0u);
+        if (qh) atomicAdd(&s.cnt[kBins + d], qh);
+        atomicAdd(&count[d], 1u);
+      });
+      if (!find_bin<true>(rem)) return false;
+      rem -= s.before;
+      const uint32_t d = s.bin;
+      const uint32_t n_bin = __reduce_add_sync(0xffffffffu, lane < p.cs ? ld32_cluster(remote(&count[d], lane)) : 0);
+      if (by_index) {
+        group = d;
+      } else {
+        key += d << shift;
+        span = (1u << shift) - 1;
+      }
+      sync();  // everybody has read the counts, which share the list's memory
+      if (n_bin > kList) continue;
+      if (tid == 0) s.n_list = 0;
+      __syncthreads();
+      each(warp_lo(), warp_hi(), floor, [&](float v, int i) { append(in(v, i), v, i); });
+      sync();
+      const uint32_t n = collect();
+      if (rank == 0) cut_in_list<true>(n, rem);
+      sync();
+      const u64 cut = p.cs > 1 ? ld64_cluster(remote(&s.cut, 0)) : s.cut;
+      sync();
+      if (tid == 0) s.cut = cut;
+      __syncthreads();
+      return true;
     }
   }
 
@@ -520,29 +631,43 @@ struct Sampler {
     // The first token of the order; the row's part into shared memory
     u64 first = ~0ull;
     float best = -INFINITY;
-    constexpr int AHEAD = 4;  // loads in flight: the pass over HBM
+    int best_e = 0;
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // maxima of a quarter of the thread's elements each
     const int hi_e = warp_hi();
-    for (int e0 = warp_lo() + lane * 8; e0 < hi_e; e0 += AHEAD * kTile) {
-      Eight r[AHEAD];
+    Eight r0, r1, r2;  // three loads ahead: the pass over HBM
+    const int e_lo = warp_lo() + lane * 8;
+    if (e_lo < hi_e) r0 = load(e_lo);
+    if (e_lo + kTile < hi_e) r1 = load(e_lo + kTile);
+    if (e_lo + 2 * kTile < hi_e) r2 = load(e_lo + 2 * kTile);
+    for (int e = e_lo; e < hi_e; e += kTile) {
+      const Eight r = r0;
+      r0 = r1;
+      r1 = r2;
+      if (e + 3 * kTile < hi_e) r2 = load(e + 3 * kTile);
+      if (p.staged) {
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        if (e0 + u * kTile < hi_e) r[u] = load(e0 + u * kTile);
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int e = e0 + u * kTile;
-        if (e >= hi_e) break;
-        if (p.staged) {
-#pragma unroll
-          for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(stage + (e - lo))[i] = reinterpret_cast<const uint4*>(r[u].t)[i];
-        }
-        const float m = max8(r[u]);
-        if (m > best) {
-          best = m;
-#pragma unroll
-          for (int j = 7; j >= 0; --j)
-            if (r[u][j] == m) first = order_of(m, e + j - skew);
-        }
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(stage + (e - lo))[i] = reinterpret_cast<const uint4*>(r.t)[i];
       }
+      const float m = max8(r);
+      if (m > best) {
+        best = m;
+        best_e = e;
+      }
+      const float mm = fmaxf(tops[0], m);  // the thread's vectors in turn
+      tops[0] = tops[1], tops[1] = tops[2], tops[2] = tops[3], tops[3] = mm;
+    }
+    // where it is, from the threads that have the CTA's largest
+    float m = best;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s.scan[warp] = __float_as_uint(m);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSW; ++w) m = fmaxf(m, __uint_as_float(static_cast<uint32_t>(s.scan[w])));
+    if (best == m && m > -INFINITY) {
+#pragma unroll 1
+      for (int j = 7; j >= 0; --j)
+        if (one(best_e + j) == best) first = order_of(best, best_e + j - skew);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
@@ -553,7 +678,9 @@ struct Sampler {
     if (p.cs > 1) {
       if (tid == 0) s.part = first;
       cluster_sync();
-      for (int c = 0; c < p.cs; ++c) first = min(first, ld64_cluster(remote(&s.part, c)));
+      if (lane < p.cs) first = ld64_cluster(remote(&s.part, lane));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
       cluster_sync();
     }
     if (first == ~0ull) {  // nothing to draw from
@@ -573,7 +700,7 @@ struct Sampler {
 
     u64 cut = ~0ull;
     if (k < p.V) {
-      if (find_cut<false>(k)) {
+      if (list_top(k, tops) || find_cut<false>(k)) {
         if (rank == 0) from_list(b, k, top_p, p24, min_p, u24);
         sync();
         return;
@@ -581,53 +708,71 @@ struct Sampler {
       cut = s.cut;
     }
     if (top_p < 1.f) {
-      // all masses, and the counts of the exponent's bins
+      // all masses
+      u64 t = 0;
+      const bool has_cut = cut != ~0ull;
+      const float cut_v = key_value(static_cast<uint32_t>(cut >> 32));
+      if (cut == ~0ull && !row.odd)
+        t = masses(0.f);
+      else
+        each(warp_lo(), warp_hi(), -INFINITY, [&](float v, int i) { t += kept(v, i, cut, 0.f); });
+      const u64 z_mass = total_of(t), limit = share(z_mass, p24, true);
+      // the counts of the exponent's bins, down to a weight of (1 - p) Z / V
       for (int i = tid; i < kBins; i += kST) s.cnt[i] = s.cnt[kBins + i] = 0;
       if (tid == 0) s.n_list = 0;
       __syncthreads();
-      u64 t = 0;
-      const float cut_v = key_value(static_cast<uint32_t>(cut >> 32));  // all ones: not a number, above nothing
+      const float least_w = static_cast<float>(z_mass - limit) * (0.99f / 1099511627776.f) / static_cast<float>(p.V);
+      const uint32_t b_end = row.odd ? kFine - 1 : whole_bins(least_w);
+      const float bulk = row.odd || b_end >= kFine - 1 ? -INFINITY : above(b_end);
       each8(warp_lo(), warp_hi(), [&](const Eight& r, int e) {
-        int hi = 0, lo8 = 0;
+        if (!(max8(r) >= bulk)) return;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float v = r[j];
-          if (v < cut_v || (v == cut_v && order_of(v, e + j - skew) > cut)) continue;
-          if (row.odd && v == -INFINITY) continue;
-          const float z = row.z(v);
-          int h, l;
-          mass_parts(row.odd ? row.w(v) : expf(z), h, l);
-          hi += h;
-          lo8 += l;
-          if (h | l) atomicAdd(&s.cnt[row.fine(v, z)], 1u);
+          if (!(v >= bulk) || v == -INFINITY) continue;
+          if (has_cut && (v < cut_v || (v == cut_v && order_of(v, e + j - skew) > cut))) continue;
+          atomicAdd(&s.cnt[row.fine(v, row.z(v))], 1u);
         }
-        t += static_cast<u64>((static_cast<long long>(hi) << 20) + lo8);
       });
-      const u64 limit = share(total_of(t), p24, true);
       find_range(limit);
       const uint32_t b_lo = s.bin, b_hi = s.bin_hi;
       // what lies surely before the cut, and a list of what may be the cut
-      const float floor = row.odd || b_hi >= kFine - 1 ? -INFINITY
-                                                       : __fsub_rn(row.m, (b_hi + 2) * (1.f / 128) / row.inv) - fabsf(row.m) * 1e-6f;
+      const float floor = row.odd || b_hi >= kFine - 1 ? -INFINITY : above(b_hi);
       u64 sure = 0, keep = 0;
-      each(warp_lo(), warp_hi(), floor, [&](float v, int i) {
-        const float z = row.z(v);
-        const uint32_t d = row.fine(v, z);
-        const bool in = !(v < cut_v || (v == cut_v && order_of(v, i) > cut)) && v > -INFINITY;
-        if (in && d < b_lo) {
-          const float w = row.w(v);
-          const u64 q = mass_of(w);
-          sure += q;
-          keep += w < min_p ? 0 : q;
+      each8(warp_lo(), warp_hi(), [&](const Eight& r, int e) {
+        if (!__any_sync(0xffffffffu, max8(r) >= floor)) return;
+        uint32_t maybe = 0;
+        int sh = 0, sl = 0, kh = 0, kl = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // without branches: most steps have something to add
+          const float v = r[j], z = row.z(v), w = row.odd ? row.w(v) : expf(z);
+          bool in = v > -INFINITY;
+          if (has_cut) in = in && !(v < cut_v || (v == cut_v && order_of(v, e + j - skew) > cut));
+          const uint32_t d = in ? row.fine(v, z) : kFine;
+          int h, l;
+          mass_parts(d < b_lo ? w : 0.f, h, l);
+          sh += h;
+          sl += l;
+          const bool k = w >= min_p;
+          kh += k ? h : 0;
+          kl += k ? l : 0;
+          maybe |= (d >= b_lo && d <= b_hi ? 1u : 0u) << j;
         }
-        append(in && d >= b_lo && d <= b_hi, v, i);
+        sure += static_cast<u64>((static_cast<long long>(sh) << 20) + sl);
+        keep += static_cast<u64>((static_cast<long long>(kh) << 20) + kl);
+        if (maybe) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) append(maybe >> j & 1, r[j], e + j - skew);
+        }
       });
       tell(keep, sure);
-      const uint32_t n = ld32_cluster(remote(&s.n_list, 0));
+      const uint32_t n = collect();
       if (n <= kList) {
         if (rank == 0) {
           u64 before = 0;
-          for (int c = 0; c < p.cs * kSW; ++c) before += s.sure[c];
+#pragma unroll
+          for (int c = 0; c < kChunks; c += 32) before += c + lane < p.cs * kSW ? s.sure[c + lane] : 0;
+          before = sum32(before);
           const bool found = before < limit && cut_in_list<true>(n, limit - before);
           if (tid == 0) s.n_bin = found;
           for (int i = tid; found && i < static_cast<int>(n); i += kST) {
@@ -638,31 +783,64 @@ struct Sampler {
           __syncthreads();
         }
         if (draw(b, u24, min_p, true)) return;
+        sync();
+      } else {  // thousands of equal or nearly equal logits at the cut
+        u64 before = 0;
+#pragma unroll
+        for (int c = 0; c < kChunks; c += 32) before += c + lane < p.cs * kSW ? ld64_cluster(remote(&s.sure[c + lane], 0)) : 0;
+        before = sum32(before);
+        sync();  // everybody has read the list's length and the sums
+        if (before < limit && cut_in_range(limit - before, b_lo, b_hi, floor)) {
+          cut = min(cut, s.cut);
+          each(warp_lo(), warp_hi(), floor, [&](float v, int i) {
+            const uint32_t d = row.fine(v, row.z(v));
+            if (d >= b_lo && d <= b_hi) keep += kept(v, i, cut, min_p);
+          });
+          if (rank == 0 && tid == 0) s.cut = cut;
+          tell(keep, 0);
+          draw(b, u24, min_p, false);
+          return;
+        }
+        sync();
       }
-      sync();  // everybody has read the list's length
       find_cut<true>(limit);
       cut = min(cut, s.cut);
     }
     u64 keep = 0;
-    if (cut == ~0ull && !row.odd) {
-      each8(warp_lo(), warp_hi(), [&](const Eight& r, int) {
-        int hi = 0, lo8 = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float w = expf(row.z(r[j]));
-          int h, l;
-          mass_parts(w < min_p ? 0.f : w, h, l);
-          hi += h;
-          lo8 += l;
-        }
-        keep += static_cast<u64>((static_cast<long long>(hi) << 20) + lo8);
-      });
-    } else {
+    if (cut == ~0ull && !row.odd)
+      keep = masses(min_p);
+    else
       each(warp_lo(), warp_hi(), -INFINITY, [&](float v, int i) { keep += kept(v, i, cut, min_p); });
-    }
     if (rank == 0 && tid == 0) s.cut = cut;
     tell(keep, 0);
     draw(b, u24, min_p, false);
+  }
+
+  // The mass of this thread's elements of the row's whole order that weigh min_p at least
+  __device__ __forceinline__ u64 masses(float min_p) const {
+    u64 t = 0;
+    const Row rw = row;
+    each8(warp_lo(), warp_hi(), [&](const Eight& r, int) {
+      int hi = 0, lo8 = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = expf(__fmul_rn(__fsub_rn(r[j], rw.m), rw.inv));
+        int h, l;
+        mass_parts(w < min_p ? 0.f : w, h, l);
+        hi += h;
+        lo8 += l;
+      }
+      t += static_cast<u64>((static_cast<long long>(hi) << 20) + lo8);
+    });
+    return t;
+  }
+  // The bin of the exponent that holds a weight, and a logit that every one of the bins up to b is above
+  __device__ __forceinline__ static uint32_t whole_bins(float w) {
+    const float t = -128.f * 0.69314718f * log2f(w) + 1.f;
+    return t >= kFine - 1 ? kFine - 1 : t > 0.f ? static_cast<uint32_t>(t) : 0u;
+  }
+  __device__ __forceinline__ float above(uint32_t b) const {
+    return __fsub_rn(row.m, (b + 2) * (1.f / 128) / row.inv) - fabsf(row.m) * 1e-6f;
   }
 
   __device__ __forceinline__ u64 kept(float v, int i, u64 cut, float min_p) const {
@@ -672,7 +850,7 @@ struct Sampler {
   }
 
   // A warp's sums to the first CTA
-  __device__ void tell(u64 keep, u64 sure) {
+  __device__ __forceinline__ void tell(u64 keep, u64 sure) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       keep += __shfl_xor_sync(0xffffffffu, keep, o);
@@ -686,7 +864,7 @@ struct Sampler {
   }
 
   // The token, from the first CTA's s.keep and s.cut; false (`check`) when s.n_bin says that there is no cut yet
-  __device__ bool draw(long long b, u64 u24, float min_p, bool check) {
+  __device__ __forceinline__ bool draw(long long b, u64 u24, float min_p, bool check) {
     if (rank == 0 && warp == 0) {
       const int n = p.cs * kSW, per = (n + 31) / 32;  // 1 to 4 chunks a lane
       u64 sum = 0;
@@ -751,7 +929,7 @@ struct Sampler {
   }
 
   // The row's total of what the threads have
-  __device__ u64 total_of(u64 mine) {
+  __device__ __forceinline__ u64 total_of(u64 mine) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) s.wsum[warp] = mine;
@@ -762,14 +940,13 @@ struct Sampler {
     if (p.cs == 1) return all;
     if (tid == 0) s.part = all;
     cluster_sync();
-    all = 0;
-    for (int c = 0; c < p.cs; ++c) all += ld64_cluster(remote(&s.part, c));
+    all = sum32(of_all(&s.part));
     cluster_sync();
     return all;
   }
 
   // The rest on the sorted list (first CTA): the first k tokens are its first k
-  __device__ void from_list(long long b, int k, float top_p, u64 p24, float min_p, u64 u24) {
+  __device__ __forceinline__ void from_list(long long b, int k, float top_p, u64 p24, float min_p, u64 u24) {
     u64 q[4], sum = 0, total;
     bool low[4];
     uint32_t idx[4];
@@ -804,7 +981,7 @@ struct Sampler {
     for (int j = 0; j < 4; ++j)
       if (tid * 4 + j < k) s.list[tid * 4 + j] = static_cast<u64>(idx[j]) << 41 | q[j];
     __syncthreads();
-    sort_list(k);
+    sort_list(s.list, k);
     sum = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -841,10 +1018,10 @@ using namespace kata;
 
 template <typename T>
 static int launch_sample(SampleParams& p, long long B, cudaStream_t st) {
-  // CTAs a row: enough to fill the GPU twice, with no fewer than two tiles a warp
+  // CTAs a row: up to two an SM, with more than a tile for each warp (1 x 131072 nucleus: 49 us on 8, 228 on one;
+  // 256 rows are as fast on one CTA each as on two)
   p.cs = 1;
-  static const int cap = getenv("SCS") ? atoi(getenv("SCS")) : 8;
-  while (p.cs < cap && B * p.cs * 2 <= 296 && p.V > p.cs * kSW * kTile) p.cs *= 2;
+  while (p.cs < 8 && B * p.cs * 2 <= 296 && p.V > p.cs * kSW * kTile) p.cs *= 2;
   const int places = p.V + 16 / static_cast<int>(sizeof(T)) - 1;
   p.seg = (places + p.cs - 1) / p.cs;
   p.seg = (p.seg + kSW * kTile - 1) / (kSW * kTile) * (kSW * kTile);
