@@ -590,7 +590,7 @@ KATA_API int kata_w4_linear(const kata_w4_weight* w, const void* x, long long ld
 /* ---------------------------------------------------------------------------------------------
  * One token per sequence between the fused q/k/v projection and kata_decode_step: causal short
  * convolution (+ SiLU) on a ring of earlier inputs, the norm of each q and k head, the rotation.
- *   a[c] = sum_{j<K} conv_w[c,j] x_{p-K+1+j}[c],  y = silu(a)   (K = 0: y = x)
+ *   a[c] = sum_{j<K} conv_w[j,c] x_{p-K+1+j}[c],  y = silu(a)   (K = 0: y = x)
  *   norm 0 none, 1 l2, 2 RMS (with q_weight / k_weight, NULL: no scale), and rope 0..2 as kata_rownorm_*
  * A row of x is [HQ heads of D | H heads of D | H heads of Dv].  ring (B, K-1, C) holds input p of a
  * sequence in slot p % (K-1) (zeros before its first token) and is updated: the slot of `positions[b]`
@@ -602,7 +602,7 @@ KATA_API int kata_w4_linear(const kata_w4_weight* w, const void* x, long long ld
  * sequences it calls fla's ShortConvolution, norms and RotaryEmbedding (kata/layer.py:296-372).
  * ------------------------------------------------------------------------------------------- */
 typedef struct {
-  const float* conv_w;    /* (C, K) fp32, C = (HQ + H) D + H Dv; NULL when K = 0 */
+  const float* conv_w;    /* (K, C) fp32, taps first, C = (HQ + H) D + H Dv, 16-byte aligned; NULL when K = 0 */
   const float* q_weight;  /* (D) fp32 or NULL */
   const float* k_weight;  /* (D) fp32 or NULL */
   const float* cos;       /* (T, R/2) fp32 or NULL */

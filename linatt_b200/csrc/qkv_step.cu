@@ -7,9 +7,11 @@
 //
 // HBM-bound: (K + 1) reads and writes of a row of inputs and one of outputs.  A thread owns eight
 // neighbouring channels; the lanes of a head are neighbours in a warp, which sums the norm and swaps
-// the halves of a rotation through shuffles.  A thread takes several sequences, so that the
-// convolution's weights are read once.  Between the steps values stay in fp32; q, k and v are rounded
-// once.
+// the halves of a rotation through shuffles.  A thread takes several sequences: the convolution's weights
+// are read once (taps first, so that lanes read neighbouring bytes), and the next sequence's inputs are on
+// their way while this one is worked on.  All slots of a ring are read in their own order, without waiting
+// for the position, which only says which weight each meets.  Between the steps values stay in fp32;
+// q, k and v are rounded once.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -40,18 +42,20 @@ struct StepParams {
 
 constexpr int kQT = 128;
 
+// Eight neighbours as they lie in memory
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&u);
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
-  } else {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ float operator[](int i) const { return to_f32<T>(reinterpret_cast<const T*>(w)[i]); }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 2) {
@@ -85,42 +89,58 @@ __global__ void __launch_bounds__(kQT) qkv_step_kernel(const StepParams p) {
   float w[K ? K : 1][8];
   if (K && live) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < K; ++j) w[j][i] = p.conv_w[static_cast<size_t>(c0 + i) * K + j];
+    for (int j = 0; j < K; ++j) {
+      const float4 lo = __ldg(reinterpret_cast<const float4*>(p.conv_w + static_cast<size_t>(j) * C + c0));
+      const float4 hi = __ldg(reinterpret_cast<const float4*>(p.conv_w + static_cast<size_t>(j) * C + c0) + 1);
+      w[j][0] = lo.x, w[j][1] = lo.y, w[j][2] = lo.z, w[j][3] = lo.w;
+      w[j][4] = hi.x, w[j][5] = hi.y, w[j][6] = hi.z, w[j][7] = hi.w;
+    }
   }
-  for (int r = 0; r < p.rows; ++r) {
-    const int b = blockIdx.y * p.rows + r;
-    if (b >= p.B) break;  // the same for the whole CTA
-    const long long pos = p.pos[b];
+  constexpr int S = K > 1 ? K - 1 : 0;  // slots of a ring
+  const int b_lo = blockIdx.y * p.rows, b_hi = min(b_lo + p.rows, p.B);
+  Eight<T> nx, no[S ? S : 1];  // the next sequence's input and ring
+  long long npos = 0;
+  auto fetch = [&](int b) {
+    npos = p.pos[b];
+    if (!live) return;
+    nx.load(static_cast<const T*>(p.x) + b * p.ldx + c0);
+#pragma unroll
+    for (int j = 0; j < S; ++j) no[j].load(static_cast<const T*>(p.ring) + (static_cast<size_t>(b) * S + j) * C + c0);
+  };
+  fetch(b_lo);
+  for (int b = b_lo; b < b_hi; ++b) {
+    const long long pos = npos;
+    const Eight<T> xin = nx;
+    Eight<T> old[S ? S : 1];
+#pragma unroll
+    for (int j = 0; j < S; ++j) old[j] = no[j];
+    if (b + 1 < b_hi) fetch(b + 1);
     const bool bad = pos < 0 || (p.rope && pos >= p.T);
-    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const T* xp = static_cast<const T*>(p.x) + b * p.ldx + c0;
-      load8<T>(xp, y);
-      if constexpr (K > 0) {
-        float xin[8];
+    float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) xin[i] = y[i];
+    for (int i = 0; i < 8; ++i) y[i] = live ? xin[i] : 0.f;
+    if (K > 0 && live) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= w[K - 1][i];
-        if constexpr (K > 1) {
-          T* rp = static_cast<T*>(p.ring) + static_cast<size_t>(b) * (K - 1) * C + c0;
-          const int at = bad ? 0 : static_cast<int>(pos % (K - 1));
+      for (int i = 0; i < 8; ++i) y[i] *= w[K ? K - 1 : 0][i];
+      if constexpr (S > 0) {
+        const int at = bad ? 0 : static_cast<int>(static_cast<unsigned long long>(pos) % S);
+        // input pos - S + j is in slot (pos + j) % S: slot s meets weight (s - at) mod S
 #pragma unroll
-          for (int j = 0; j < K - 1; ++j) {  // input pos - (K - 1) + j is in slot (pos + j) % (K - 1)
-            int sl = at + j;
-            if (sl >= K - 1) sl -= K - 1;
-            float o[8];
-            load8<T>(rp + static_cast<size_t>(sl) * C, o);
+        for (int s = 0; s < S; ++s) {
+          int j = s - at;
+          if (j < 0) j += S;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = fmaf(w[j][i], o[i], y[i]);
+          for (int i = 0; i < 8; ++i) {
+            float wj = w[0][i];
+#pragma unroll
+            for (int t = 1; t < S; ++t) wj = j == t ? w[t][i] : wj;
+            y[i] = fmaf(wj, old[s][i], y[i]);
           }
-          if (!bad) store8<T>(rp + static_cast<size_t>(at) * C, xin);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] / (1.f + expf(-y[i]));
+        if (!bad) xin.store(static_cast<T*>(p.ring) + (static_cast<size_t>(b) * S + at) * C + c0);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fdividef(y[i], 1.f + __expf(-y[i]));  // as kata_short_conv_fwd
     }
     if (p.norm_q | p.norm_k) {  // the same for the whole warp, whose heads may be of all three kinds
       float ss = 0.f;
@@ -207,7 +227,7 @@ extern "C" int kata_qkv_step(const kata_qkv_step_args* a, const void* x, long lo
   if (B == 0) return KATA_OK;
   if (!x || !positions || !q || !k || !v || (a->K > 1 && !ring)) return KATA_ERR_INVALID;
   auto al = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; };
-  if (!al(x) || !al(q) || !al(k) || !al(v) || (a->K > 1 && !al(ring)) || ldx % (a->dtype == KATA_DTYPE_F32 ? 4 : 8))
+  if (!al(a->conv_w) || !al(x) || !al(q) || !al(k) || !al(v) || (a->K > 1 && !al(ring)) || ldx % (a->dtype == KATA_DTYPE_F32 ? 4 : 8))
     return KATA_ERR_ALIGN;
   StepParams p;
   p.x = x;
@@ -237,9 +257,10 @@ extern "C" int kata_qkv_step(const kata_qkv_step_args* a, const void* x, long lo
   int lph = 1;
   while (lph * 8 < std::max(a->D, a->Dv)) lph *= 2;
   p.lph = lph;
-  // more sequences than that per CTA once the grid fills the GPU several times over
+  // several sequences a thread once the grid fills the GPU several times over (1024 x 6144: 31.3 us with one, 25.6
+  // with three or more)
   const long long ctas = ((a->HQ + 2ll * a->H) * lph + kQT - 1) / kQT * B;
-  p.rows = static_cast<int>(std::max<long long>(std::min<long long>(8, ctas / (148 * 8)), (B + 65534) / 65535));
+  p.rows = static_cast<int>(std::max<long long>(std::min<long long>(4, ctas / (148 * 8)), (B + 65534) / 65535));
   p.rows = std::max(p.rows, 1);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a->dtype == KATA_DTYPE_BF16)

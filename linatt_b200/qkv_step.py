@@ -66,6 +66,8 @@ class QKVStep:
                     or cos.shape[0] < 1:
                 raise ValueError(f"cos and sin must be (positions, {rope_dim // 2})")
             T = cos.shape[0]
+        if conv_weight is not None:
+            conv_weight = conv_weight.detach().reshape(C, self.conv_size).T  # taps first, as the kernel reads them
         self._keep = [f32(t) for t in (conv_weight, q_weight, k_weight, cos, sin)]
         self._args = {dt: _lib.QkvStepArgs(*[_lib.ptr(t) for t in self._keep], code, num_heads, H, head_k_dim, head_v_dim,
                                            self.conv_size, _NORM[norm_q], _NORM[norm_k], rope, rope_dim, T, eps_q, eps_k)
