@@ -1003,8 +1003,8 @@ int launch_gemm(const kata_w4_weight* w, const void* x, long long ldx, long long
   p.zeros = w->zeros;
   p.g = w4_geom(w);
   const int blocks = (p.g.tiles + 7) / 8, slabs = (rows + R - 1) / R;
-  p.cs = 1;
-  while (p.cs < 8 && blocks * slabs * p.cs * 2 <= 148 && p.g.steps >= 4 * p.cs) p.cs *= 2;
+  // CTAs that split k, as many as the GPU has room for, with two steps each at least
+  p.cs = std::max(1, std::min(std::min(8, 148 / (blocks * slabs)), p.g.steps / 2));
   CUtensorMap tm;
   const uint64_t dims[3] = {static_cast<uint64_t>(w->K), static_cast<uint64_t>(rows), PARTS};
   const uint64_t str[2] = {static_cast<uint64_t>(ldx) * 2, static_cast<uint64_t>(PARTS == 1 ? ldx * rows : plane) * 2};
@@ -1060,11 +1060,13 @@ int w4_check(const kata_w4_weight* w) {
 
 // Rows that are streamed over.  Up to 16 columns (5 rows, 4 of fp32) the streaming kernel is ahead whatever the
 // size (5 x 8192 x 8192: 20.6 against 23.9 us); up to 32 only while a weight is small and the fixed cost counts
-// (8 x 768 x 768: 5.1 against 9.7 us; 8 x 4096 x 4096: 14.9 against 13.8 us).
-int stream_rows(const kata_w4_weight* w) {
+// (8 x 768 x 768: 5.1 against 9.7 us; 8 x 4096 x 4096: 14.9 against 13.8 us), or where 16-bit rows would have to be
+// laid out for TMA first (7 x 4100 x 5003: 20.2 against 26.6 us).
+int stream_rows(const kata_w4_weight* w, const void* x, long long ldx) {
   const W4Geom g = w4_geom(w);
   const bool small = static_cast<long long>(g.tiles) * g.steps <= 4096;
-  return w->dtype == KATA_DTYPE_F32 ? (small ? 8 : 4) : (small ? 10 : 5);
+  if (w->dtype == KATA_DTYPE_F32) return small ? 8 : 4;
+  return small || !tma_ready(w->dtype, x, ldx) ? 10 : 5;
 }
 size_t w4_esize(int dtype) { return dtype == KATA_DTYPE_F32 ? 4 : 2; }
 bool w4_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -1101,7 +1103,7 @@ extern "C" int kata_w4_pack(const void* packed, const void* scales, const void* 
 }
 
 extern "C" size_t kata_w4_workspace_bytes(const kata_w4_weight* w, const void* x, long long ldx, long long rows) {
-  if (w4_check(w) || rows <= stream_rows(w) || tma_ready(w->dtype, x, ldx)) return 0;
+  if (w4_check(w) || rows <= stream_rows(w, x, ldx) || tma_ready(w->dtype, x, ldx)) return 0;
   return static_cast<size_t>(rows) * ((w->K + 7) / 8 * 8) * (w->dtype == KATA_DTYPE_F32 ? 6 : 2);
 }
 
@@ -1121,7 +1123,7 @@ extern "C" int kata_w4_linear(const kata_w4_weight* w, const void* x, long long 
   if (need && !w4_al16(workspace)) return KATA_ERR_ALIGN;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int n = static_cast<int>(rows);
-  if (rows <= stream_rows(w)) {
+  if (rows <= stream_rows(w, x, ldx)) {
     if (w->dtype == KATA_DTYPE_BF16) return launch_rows<__nv_bfloat16>(w, x, ldx, y, ldy, n, status, st);
     if (w->dtype == KATA_DTYPE_F16) return launch_rows<__half>(w, x, ldx, y, ldy, n, status, st);
     return launch_rows<float>(w, x, ldx, y, ldy, n, status, st);

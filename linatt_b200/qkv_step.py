@@ -87,33 +87,35 @@ class QKVStep:
                 ring[:, p % ring.shape[1]] = x[:, p]
         return ring
 
-    @torch.no_grad()
     def __call__(self, qkv: torch.Tensor, positions: torch.Tensor, ring: torch.Tensor | None = None):
         """q (B, num_heads, head_k_dim), k (B, num_kv_heads, head_k_dim), v (B, num_kv_heads, head_v_dim) of the
         projections qkv (B, C) of the tokens at ``positions`` (B,) int64.  ``ring`` (B, K - 1, C) is updated in place.
         A position that is negative or past the rotation tables gives NaN."""
         dev = _lib.require_cuda(qkv, positions, ring)
-        if qkv.dim() != 2 or qkv.shape[1] != self.channels:
-            raise ValueError(f"qkv must be (B, {self.channels}), got {tuple(qkv.shape)}")
-        dt = qkv.dtype
-        if dt not in self._args:
+        dt, shape = qkv.dtype, qkv.shape
+        if len(shape) != 2 or shape[1] != self.channels:
+            raise ValueError(f"qkv must be (B, {self.channels}), got {tuple(shape)}")
+        args = self._args.get(dt)
+        if args is None:
             raise TypeError(f"unsupported dtype {dt}")
-        B = qkv.shape[0]
+        B = shape[0]
         if positions.shape != (B,) or positions.dtype != torch.int64:
             raise ValueError(f"positions must be ({B},) int64, got {tuple(positions.shape)} {positions.dtype}")
-        if self.conv_size > 1:
-            if ring is None or ring.shape != (B, self.conv_size - 1, self.channels) or ring.dtype != dt or \
-                    not ring.is_contiguous():
-                raise ValueError(f"ring must be a contiguous ({B}, {self.conv_size - 1}, {self.channels}) {dt} tensor")
-        if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) < self.channels or qkv.data_ptr() % 16:
-            qkv = qkv.contiguous() if qkv.data_ptr() % 16 == 0 or not qkv.is_contiguous() else qkv.clone()
+        if self.conv_size > 1 and (ring is None or ring.shape != (B, self.conv_size - 1, self.channels) or
+                                   ring.dtype != dt or not ring.is_contiguous()):
+            raise ValueError(f"ring must be a contiguous ({B}, {self.conv_size - 1}, {self.channels}) {dt} tensor")
+        ld, one = qkv.stride()
+        if one != 1 or ld % 8 or ld < self.channels or qkv.data_ptr() % 16:
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
+            ld = self.channels
+        if positions.stride(0) != 1:
+            positions = positions.contiguous()
         q = torch.empty(B, self.num_heads, self.head_k_dim, dtype=dt, device=dev)
         k = torch.empty(B, self.num_kv_heads, self.head_k_dim, dtype=dt, device=dev)
         v = torch.empty(B, self.num_kv_heads, self.head_v_dim, dtype=dt, device=dev)
         with _lib.on_device(dev):
-            rc = _lib.lib().kata_qkv_step(self._args[dt], qkv.data_ptr(), qkv.stride(0), positions.contiguous().data_ptr(),
-                                          _lib.ptr(ring), q.data_ptr(), k.data_ptr(), v.data_ptr(), B,
-                                          _lib.stream_handle(dev))
+            rc = _lib.lib().kata_qkv_step(args, qkv.data_ptr(), ld, positions.data_ptr(), _lib.ptr(ring), q.data_ptr(),
+                                          k.data_ptr(), v.data_ptr(), B, _lib.stream_handle(dev))
         if rc:
             _lib.check(rc, "kata_qkv_step")
         return q, k, v

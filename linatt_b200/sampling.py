@@ -20,8 +20,10 @@ __all__ = ["sample_tokens"]
 
 def _setting(v, name, dtype, B, dev):
     """(tensor or None, scalar) of a setting given as a number or as a (B,) tensor."""
-    if not isinstance(v, torch.Tensor):
+    if type(v) in (int, float):
         return None, v
+    if not isinstance(v, torch.Tensor):
+        return None, float(v)
     if v.shape != (B,):
         raise ValueError(f"{name} must be a number or a ({B},) tensor, got {tuple(v.shape)}")
     if v.device != dev:
@@ -29,7 +31,6 @@ def _setting(v, name, dtype, B, dev):
     return v.to(dtype).contiguous(), 0
 
 
-@torch.no_grad()
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
                   min_p=0.0) -> tuple[torch.Tensor, torch.Tensor]:
     """(token (B,) int64, logprob (B,) fp32) drawn from logits (B, V) bf16 / f16 / fp32 with the uniform
@@ -43,22 +44,27 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     if logits.dtype not in _lib.DTYPE:
         raise TypeError(f"unsupported logits dtype {logits.dtype}")
     B, V = logits.shape
+    ld, one = logits.stride()
     if u.shape != (B,) or u.dtype != torch.float32:
         raise ValueError(f"u must be ({B},) fp32, got {tuple(u.shape)} {u.dtype}")
     if V < 1:
         raise ValueError("the vocabulary is empty")
-    if logits.stride(1) != 1 or (logits.stride(0) < V and B > 1):
+    if one != 1 or (ld < V and B > 1):
         logits = logits.contiguous()
+        ld = V
     tt, ts = _setting(temperature, "temperature", torch.float32, B, dev)
     kt, ks = _setting(top_k, "top_k", torch.int32, B, dev)
     pt, ps = _setting(top_p, "top_p", torch.float32, B, dev)
     mt, ms = _setting(min_p, "min_p", torch.float32, B, dev)
-    u = u.contiguous()
+    if u.stride(0) != 1:
+        u = u.contiguous()
     token = torch.empty(B, dtype=torch.int64, device=dev)
     logprob = torch.empty(B, dtype=torch.float32, device=dev)
     a = _lib.SampleArgs(logits.data_ptr(), u.data_ptr(), _lib.ptr(tt), _lib.ptr(kt), _lib.ptr(pt), _lib.ptr(mt),
-                        token.data_ptr(), logprob.data_ptr(), logits.stride(0), B, V, _lib.DTYPE[logits.dtype], ts,
+                        token.data_ptr(), logprob.data_ptr(), ld, B, V, _lib.DTYPE[logits.dtype], ts,
                         min(max(int(ks), 0), 2 ** 31 - 1), ps, ms)
     with _lib.on_device(dev):
-        _lib.check(_lib.lib().kata_sample(a, _lib.stream_handle(dev)), "kata_sample")
+        rc = _lib.lib().kata_sample(a, _lib.stream_handle(dev))
+    if rc:
+        _lib.check(rc, "kata_sample")
     return token, logprob
