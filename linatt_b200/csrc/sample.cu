@@ -563,26 +563,38 @@ struct Sampler {
     // a logit above all of the range: the slack of `above` the other way
     const float ceil = row.odd || b_lo < 3 ? INFINITY : __fsub_rn(row.m, (b_lo - 2) * (1.f / 128) / row.inv) + fabsf(row.m) * 1e-6f;
     uint32_t key = order_key(ceil), span = order_key(floor) - key;  // keys key .. key + span
-    int group = -1;                                                 // of 2048 indexes
+    int group = -1, places = 3;                                     // of 2^places places, at most 2048
+    while ((p.V + 8) >> places >= kBins) ++places;
     uint32_t* count = reinterpret_cast<uint32_t*>(s.list);
     for (;;) {
       const int shift = max(0, 21 - __clz(span));  // span >> shift < 2048
       const bool by_index = span == 0;
       auto in = [&](float v, int i) {
         const uint32_t d = row.fine(v, row.z(v));
-        return v >= floor && v > -INFINITY && d >= b_lo && d <= b_hi && order_key(v) - key <= span && (group < 0 || i >> 11 == group);
+        return v >= floor && v > -INFINITY && d >= b_lo && d <= b_hi && order_key(v) - key <= span && (group < 0 || (i + skew) >> places == group);
       };
       for (int i = tid; i < kBins; i += kST) s.cnt[i] = s.cnt[kBins + i] = count[i] = 0;
       __syncthreads();
-      each(warp_lo(), warp_hi(), floor, [&](float v, int i) {
-        if (!in(v, i)) return;
-        const uint32_t d = by_index ? i >> 11 : (order_key(v) - key) >> shift;
-        const u64 q = mass_of(row.w(v));
+      auto add = [&](uint32_t d, u64 q, uint32_t n) {
         const uint32_t ql = static_cast<uint32_t>(q), old = atomicAdd(&s.cnt[d], ql);
         const uint32_t qh = static_cast<uint32_t>(q >> 32) + (old + ql < old ? 1u : 0u);
         if (qh) atomicAdd(&s.cnt[kBins + d], qh);
-        atomicAdd(&count[d], 1u);
-      });
+        atomicAdd(&count[d], n);
+      };
+      if (by_index) {  // one logit: a thread's eight neighbours at once
+        const u64 q = mass_of(row.w(key_value(key)));
+        each8(warp_lo(), warp_hi(), [&](const Eight& r, int e) {
+          if (!(max8(r) >= floor)) return;
+          uint32_t n = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) n += in(r[j], e + j - skew);
+          if (n) add(e >> places, n * q, n);
+        });
+      } else {
+        each(warp_lo(), warp_hi(), floor, [&](float v, int i) {
+          if (in(v, i)) add((order_key(v) - key) >> shift, mass_of(row.w(v)), 1);
+        });
+      }
       if (!find_bin<true>(rem)) return false;
       rem -= s.before;
       const uint32_t d = s.bin;
@@ -633,28 +645,46 @@ struct Sampler {
     float best = -INFINITY;
     int best_e = 0;
     float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // maxima of a quarter of the thread's elements each
-    const int hi_e = warp_hi();
-    Eight r0, r1, r2;  // three loads ahead: the pass over HBM
-    const int e_lo = warp_lo() + lane * 8;
-    if (e_lo < hi_e) r0 = load(e_lo);
-    if (e_lo + kTile < hi_e) r1 = load(e_lo + kTile);
-    if (e_lo + 2 * kTile < hi_e) r2 = load(e_lo + 2 * kTile);
-    for (int e = e_lo; e < hi_e; e += kTile) {
-      const Eight r = r0;
-      r0 = r1;
-      r1 = r2;
-      if (e + 3 * kTile < hi_e) r2 = load(e + 3 * kTile);
+    const int hi_e = warp_hi(), e_lo = warp_lo() + lane * 8;
+    auto take = [&](const Eight& r, int e, bool before) {
       if (p.staged) {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(stage + (e - lo))[i] = reinterpret_cast<const uint4*>(r.t)[i];
       }
       const float m = max8(r);
-      if (m > best) {
+      if (m > best || (before && m == best)) {
         best = m;
         best_e = e;
       }
-      const float mm = fmaxf(tops[0], m);  // the thread's vectors in turn
-      tops[0] = tops[1], tops[1] = tops[2], tops[2] = tops[3], tops[3] = mm;
+      return m;
+    };
+    constexpr int AHEAD = sizeof(T) == 2 ? 8 : 4;  // loads in flight: the pass over HBM
+#pragma unroll 1
+    for (int e0 = e_lo; e0 < hi_e; e0 += AHEAD * kTile) {
+      Eight r[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int e = e0 + u * kTile;
+        if (e < hi_e && e >= skew && e + 8 <= skew + p.V) {
+#pragma unroll
+          for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+            reinterpret_cast<uint4*>(r[u].t)[i] = __ldg(reinterpret_cast<const uint4*>(x + (e - skew)) + i);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) r[u].t[j] = from_f32<T>(-INFINITY);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (e0 + u * kTile < hi_e) tops[u & 3] = fmaxf(tops[u & 3], take(r[u], e0 + u * kTile, false));
+      }
+    }
+    // the row's first and last eight, where they are not whole
+#pragma unroll 1
+    for (int end = 0; end < 2; ++end) {
+      const int e = end ? (skew + p.V) / 8 * 8 : 0;
+      const bool whole = end ? (skew + p.V) % 8 == 0 || (e == 0 && skew > 0) : skew == 0;
+      if (!whole && e >= e_lo && e < hi_e && (e - e_lo) % kTile == 0) tops[0] = fmaxf(tops[0], take(load_edge(e), e, end == 0));
     }
     // where it is, from the threads that have the CTA's largest
     float m = best;

@@ -142,6 +142,19 @@ def test_sampling_equal_logits_go_by_index(par):
     check(signed, u, **par)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [9, 1001, 40003])
+def test_sampling_equal_logits_in_rows_off_16_bytes(V, dtype):
+    """Rows that start between 16-byte boundaries: their first and last logits tie with others."""
+    u = torch.tensor([0.0, 0.3, 0.6, 0.9, 0.99999994], device="cuda")
+    x = torch.full((5, V), 2.0, device="cuda", dtype=dtype)
+    for par in (dict(temperature=0.0), dict(top_k=1), dict(top_k=3), dict(top_p=0.5), dict(top_k=V - 2, top_p=0.9)):
+        check(x, u, **par)
+        y = x.clone()
+        y[:, 1:-1] = 1.0  # only the ends
+        check(y, u, **par)
+
+
 def test_sampling_close_logits_share_a_histogram_bin():
     """fp32 logits that differ in their last bits only: the cut is found by their bits."""
     base = torch.tensor(5.0).view(torch.int32).item()
