@@ -1048,10 +1048,13 @@ using namespace kata;
 
 template <typename T>
 static int launch_sample(SampleParams& p, long long B, cudaStream_t st) {
-  // CTAs a row: up to two an SM, with more than a tile for each warp (1 x 131072 nucleus: 49 us on 8, 228 on one;
-  // 256 rows are as fast on one CTA each as on two)
+  // CTAs a row: up to two an SM, with more than a tile for each warp (1 x 131072 nucleus: 49 us on 8, 228 on one).
+  // Rows of their own settings differ several times in cost, and with one CTA each the last one is waited for: long
+  // ones get twice as many (256 x 131072: 234 against 369 us; with one setting for all, 264 against 223).
+  const bool differ = p.temperature || p.top_k || p.top_p || p.min_p;
+  const long long room = differ && p.V >= 65536 ? 592 : 296;
   p.cs = 1;
-  while (p.cs < 8 && B * p.cs * 2 <= 296 && p.V > p.cs * kSW * kTile) p.cs *= 2;
+  while (p.cs < 8 && B * p.cs * 2 <= room && p.V > p.cs * kSW * kTile) p.cs *= 2;
   const int places = p.V + 16 / static_cast<int>(sizeof(T)) - 1;
   p.seg = (places + p.cs - 1) / p.cs;
   p.seg = (p.seg + kSW * kTile - 1) / (kSW * kTile) * (kSW * kTile);
