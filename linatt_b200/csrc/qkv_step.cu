@@ -12,6 +12,10 @@
 // their way while this one is worked on.  All slots of a ring are read in their own order, without waiting
 // for the position, which only says which weight each meets.  Between the steps values stay in fp32;
 // q, k and v are rounded once.
+//
+// Measured (device time): 1024 x 6144 bf16 with K = 4, RMS and rotation in 24.4 us, 3.1 TB/s (0.48 of the measured copy
+// rate); 1 x 2304 in 2.2 us, an empty launch.  Bound by latency at 500 threads an SM: with 80 or 64 registers a
+// thread there are more, but they spill (35 and 53 us).
 #include <algorithm>
 
 #include "attn_common.cuh"
