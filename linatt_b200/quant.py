@@ -93,12 +93,13 @@ def w4_linear(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
     y = torch.empty(*shape[:-1], w.out_features, dtype=w.dtype, device=dev)
     if rows:
         with _lib.on_device(dev):
-            L, ws, n = _lib.lib(), None, 0
-            if rows > 1:  # one row never needs any
-                n = L.kata_w4_workspace_bytes(w._args, x2.data_ptr(), ldx, rows)
+            L, xp, ws, n = _lib.lib(), x2.data_ptr(), None, 0
+            # four rows, and 16-bit ones that lie on 16-byte boundaries, never need any
+            if rows > 4 and (w.dtype is torch.float32 or ldx % 8 or xp % 16):
+                n = L.kata_w4_workspace_bytes(w._args, xp, ldx, rows)
                 if n:
                     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            rc = L.kata_w4_linear(w._args, x2.data_ptr(), ldx, y.data_ptr(), w.out_features, rows, _lib.ptr(ws), n,
+            rc = L.kata_w4_linear(w._args, xp, ldx, y.data_ptr(), w.out_features, rows, _lib.ptr(ws), n,
                                   _lib.status_word(dev).data_ptr(), _lib.stream_handle(dev))
         if rc:
             _lib.check(rc, "kata_w4_linear")
