@@ -48,6 +48,7 @@ constexpr int kList = 2048;          // elements sorted directly
 constexpr int kFine = 2 * kBins;     // bins of the exponent
 constexpr int kChunks = 8 * kSW;     // warps of a row
 constexpr int kTile = 256;           // elements a warp takes at once: 8 a lane
+constexpr int kMaxV = 1 << 22;       // find_cut has 22 bits of the index, from_list packs as many beside a mass
 constexpr int kStage = 96 * 1024;    // bytes of a part of a row that are kept in shared memory
 typedef unsigned long long u64;
 
@@ -158,6 +159,15 @@ __device__ __forceinline__ u64 share(u64 total, u64 n24, bool up) {
   const u64 hi = __umul64hi(total, n24), lo = total * n24;
   return (hi << 40) + (lo >> 24) + ((up && (lo & 0xffffffull)) ? 1 : 0);
 }
+
+// The digit of a place in a range of width + 1: (place - first) >> shift is below kBins, and eight neighbours share one
+__host__ __device__ constexpr int index_shift(uint32_t width) {
+  int shift = 3;
+  while (width >> shift >= kBins) ++shift;
+  return shift;
+}
+// Two digits leave no more places than the list holds, whatever the row's length and alignment
+static_assert((1 << index_shift((1u << index_shift(kMaxV + 7)) - 1)) <= kList, "digits of places");
 
 // Ascending sort of n different numbers by the CTA.  Up to one a thread: each finds its rank (8 cycles a number);
 // beyond that by merging (66 steps of 300 cycles for 2048).
@@ -565,16 +575,18 @@ struct Sampler {
   __device__ __forceinline__ bool cut_in_range(u64 rem, uint32_t b_lo, uint32_t b_hi, float floor) {
     // a logit above all of the range: the slack of `above` the other way
     const float ceil = row.odd || b_lo < 3 ? INFINITY : __fsub_rn(row.m, (b_lo - 2) * (1.f / 128) / row.inv) + fabsf(row.m) * 1e-6f;
-    uint32_t key = order_key(ceil), span = order_key(floor) - key;  // keys key .. key + span
-    int group = -1, places = 3;                                     // of 2^places places, at most 2048
-    while ((p.V + 8) >> places >= kBins) ++places;
+    uint32_t key = order_key(ceil), span = order_key(floor) - key;    // keys key .. key + span
+    uint32_t place = 0, width = static_cast<uint32_t>(p.V + skew - 1);  // places place .. place + width
     uint32_t* count = reinterpret_cast<uint32_t*>(s.list);
+    // Each round takes a digit of the keys, or once one is left, of the places, and narrows their range to the digit's:
+    // three of the keys at most, and two of the places, since V <= kMaxV and a digit of the lowest three bits, eight
+    // neighbours, always fits the list.
     for (;;) {
-      const int shift = max(0, 21 - __clz(span));  // span >> shift < 2048
       const bool by_index = span == 0;
+      const int shift = by_index ? index_shift(width) : max(0, 21 - __clz(span));  // span >> shift < 2048
       auto in = [&](float v, int i) {
         const uint32_t d = row.fine(v, row.z(v));
-        return v >= floor && v > -INFINITY && d >= b_lo && d <= b_hi && order_key(v) - key <= span && (group < 0 || (i + skew) >> places == group);
+        return v >= floor && v > -INFINITY && d >= b_lo && d <= b_hi && order_key(v) - key <= span && i + skew - place <= width;
       };
       for (int i = tid; i < kBins; i += kST) s.cnt[i] = s.cnt[kBins + i] = count[i] = 0;
       __syncthreads();
@@ -591,7 +603,7 @@ struct Sampler {
           uint32_t n = 0;
 #pragma unroll
           for (int j = 0; j < 8; ++j) n += in(r[j], e + j - skew);
-          if (n) add(e >> places, n * q, n);
+          if (n) add((e - place) >> shift, n * q, n);
         });
       } else {
         each(warp_lo(), warp_hi(), floor, [&](float v, int i) {
@@ -603,7 +615,8 @@ struct Sampler {
       const uint32_t d = s.bin;
       const uint32_t n_bin = __reduce_add_sync(0xffffffffu, lane < p.cs ? ld32_cluster(remote(&count[d], lane)) : 0);
       if (by_index) {
-        group = d;
+        place += d << shift;
+        width = (1u << shift) - 1;
       } else {
         key += d << shift;
         span = (1u << shift) - 1;
@@ -1085,7 +1098,7 @@ static int launch_sample(SampleParams& p, long long B, cudaStream_t st) {
 extern "C" int kata_sample(const kata_sample_args* a, kata_stream_t stream) {
   if (!a) return KATA_ERR_INVALID;
   if (a->dtype != KATA_DTYPE_F32 && a->dtype != KATA_DTYPE_BF16 && a->dtype != KATA_DTYPE_F16) return KATA_ERR_DTYPE;
-  if (a->B < 0 || a->V < 1 || a->B > (1ll << 28) || a->V > (1 << 22)) return KATA_ERR_SHAPE;
+  if (a->B < 0 || a->V < 1 || a->B > (1ll << 28) || a->V > kMaxV) return KATA_ERR_SHAPE;
   if (a->B > 1 && a->ld < a->V) return KATA_ERR_SHAPE;
   if (a->B == 0) return KATA_OK;
   if (!a->logits || !a->u || !a->token || !a->logprob) return KATA_ERR_INVALID;

@@ -142,6 +142,27 @@ def test_sampling_equal_logits_go_by_index(par):
     check(signed, u, **par)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [4194295, 4194296, 4194301, 4194304])
+@pytest.mark.parametrize("skew,step", [(0, 1), (3, 1), (0, 1500), (1, 2)])
+def test_sampling_equal_logits_at_the_largest_vocabularies(V, dtype, skew, step):
+    """A nucleus cut among millions of equal logits, or thousands that are the same number of places apart: the
+    first n of them are kept, n the least with n / count >= p, and u picks one of these."""
+    from linatt_b200.sampling import sample_tokens
+
+    u = torch.tensor([0.0, 0.37, 0.99999994], device="cuda")
+    buf = torch.full((3, V + skew), -40.0, device="cuda", dtype=dtype)
+    x = buf[:, skew:]
+    x[:, ::step] = 1.5
+    count = -(-V // step)
+    for top_p in (0.0001, 0.5, 0.9):
+        p24 = int(torch.tensor(top_p, dtype=torch.float32).item() * 2 ** 24)
+        n = -(-p24 * count // 2 ** 24)
+        token, logprob = sample_tokens(x, u, top_p=top_p)
+        assert token.tolist() == [(int(v * 2 ** 24) * n >> 24) * step for v in u.tolist()]
+        assert (logprob.double() + math.log(n)).abs().max() <= 2.0 ** -23 * math.log(count)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("V", [9, 1001, 40003])
 def test_sampling_equal_logits_in_rows_off_16_bytes(V, dtype):
