@@ -98,11 +98,12 @@ class AddRMSNormFunction(torch.autograd.Function):
         h_out = torch.empty_like(hc)
         y = torch.empty(xc.shape, device=dev, dtype=xc.dtype)
         rstd = torch.empty(rows, device=dev, dtype=torch.float32)
-        a = _lib.AddRmsNormArgs(h=hc.data_ptr(), x=xc.data_ptr(), w=w.data_ptr(), h_out=h_out.data_ptr(),
+        wf = w.detach().float().contiguous()  # the kernels read fp32, whatever the parameter's type
+        a = _lib.AddRmsNormArgs(h=hc.data_ptr(), x=xc.data_ptr(), w=wf.data_ptr(), h_out=h_out.data_ptr(),
                                 y=y.data_ptr(), rstd=rstd.data_ptr(), rows=rows, N=N, dtype=_dt(xc), eps=float(eps))
         _lib.check(_lib.lib().kata_add_rmsnorm_fwd(a, _lib.stream_handle(dev)), "kata_add_rmsnorm_fwd")
-        ctx.save_for_backward(h_out, rstd, w)
-        ctx.eps, ctx.xdtype = eps, xc.dtype
+        ctx.save_for_backward(h_out, rstd, wf)
+        ctx.eps, ctx.xdtype, ctx.wdtype = eps, xc.dtype, w.dtype
         return h_out, y
 
     @staticmethod
@@ -124,7 +125,7 @@ class AddRMSNormFunction(torch.autograd.Function):
         ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nb
         _lib.check(L.kata_add_rmsnorm_bwd(a, _lib.stream_handle(dev)), "kata_add_rmsnorm_bwd")
-        return dh, dx, dw, None
+        return dh, dx, dw.to(ctx.wdtype), None
 
 
 def add_rmsnorm(h: torch.Tensor, x: torch.Tensor, norm: "RMSNorm"):

@@ -66,6 +66,24 @@ def test_a_prompt_is_the_lm_with_rounded_weights():
     assert rel(got, want) < 3e-2
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_converted_model_generates_as_its_own_values(dtype):
+    """Parameters in 16 bits: the same as fp32 parameters of the same values."""
+    from linatt_b200.generate import KataGenerator
+
+    lm = make(use_rope=True, qk_norm=True).to(dtype)
+    for p in lm.parameters():
+        if p.dim() == 1:  # norm weights that differ
+            torch.nn.init.uniform_(p, 0.5, 1.5)
+    ids = torch.randint(0, 512, (3, 20), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    gen = KataGenerator(lm, dtype=dtype)
+    got = [gen.prefill(ids[:, :19]), gen.step(ids[:, 19])]
+    gen = KataGenerator(lm.float(), dtype=dtype)
+    want = [gen.prefill(ids[:, :19]), gen.step(ids[:, 19])]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("head", [False, True])
 def test_generate_captured_and_not(head):
     from linatt_b200 import check_device_status
