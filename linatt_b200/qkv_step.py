@@ -34,7 +34,7 @@ class QKVStep:
                  q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps_q: float = 1e-5,
                  eps_k: float = 1e-5, rope: int = 0, rope_dim: int = 0, cos: torch.Tensor | None = None,
                  sin: torch.Tensor | None = None):
-        _lib.require_cuda(conv_weight, q_weight, k_weight, cos, sin)
+        self.device = _lib.require_cuda(conv_weight, q_weight, k_weight, cos, sin)  # None: nothing is kept
         H = num_heads if num_kv_heads is None else num_kv_heads
         if H < 1 or num_heads % H:
             raise ValueError(f"num_heads={num_heads} must be a multiple of num_kv_heads={H}")
@@ -92,6 +92,8 @@ class QKVStep:
         projections qkv (B, C) of the tokens at ``positions`` (B,) int64.  ``ring`` (B, K - 1, C) is updated in place.
         A position that is negative or past the rotation tables gives NaN."""
         dev = _lib.require_cuda(qkv, positions, ring)
+        if self.device is not None and dev != self.device:
+            raise RuntimeError(f"qkv is on {dev}, the weights and tables on {self.device}")
         dt, shape = qkv.dtype, qkv.shape
         if len(shape) != 2 or shape[1] != self.channels:
             raise ValueError(f"qkv must be (B, {self.channels}), got {tuple(shape)}")

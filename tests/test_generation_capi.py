@@ -106,3 +106,28 @@ def test_fronts_refuse_cpu_tensors():
         QKVStep(num_heads=1, head_k_dim=8, head_v_dim=8, conv_weight=torch.zeros(24, 4))
     with pytest.raises(RuntimeError):
         sample_tokens(torch.zeros(2, 10), torch.zeros(2))
+
+
+def test_qkv_step_refuses_inputs_on_another_device_than_its_weights(monkeypatch):
+    """On the host, without a launch: the devices are stated, not looked up."""
+    from linatt_b200 import qkv_step
+
+    def on(i):
+        monkeypatch.setattr(_lib, "require_cuda", lambda *ts: None if all(t is None for t in ts) else torch.device("cuda", i))
+
+    class Never:
+        def kata_qkv_step(self, *a):
+            raise AssertionError("launched")
+
+    monkeypatch.setattr(_lib, "lib", lambda: Never())
+    on(0)
+    step = qkv_step.QKVStep(num_heads=1, head_k_dim=8, head_v_dim=8, conv_weight=torch.zeros(24, 1))
+    free = qkv_step.QKVStep(num_heads=1, head_k_dim=8, head_v_dim=8)
+    on(1)
+    with pytest.raises(RuntimeError, match="cuda:1.*cuda:0"):
+        step(torch.zeros(2, 24), torch.zeros(2, dtype=torch.int64))
+    monkeypatch.setattr(_lib, "on_device", lambda dev: _lib._STAY)
+    monkeypatch.setattr(_lib, "stream_handle", lambda dev: 0)
+    monkeypatch.setattr(torch, "empty", lambda *s, dtype, device: torch.zeros(*s, dtype=dtype))
+    with pytest.raises(AssertionError, match="launched"):  # without weights there is nothing to be elsewhere
+        free(torch.zeros(2, 24), torch.zeros(2, dtype=torch.int64))
