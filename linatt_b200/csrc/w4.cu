@@ -87,17 +87,24 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint32_t* __restrict
 //
 // Turning codes into 16-bit floats costs 11 instructions a word and bounds such a kernel at half the HBM
 // rate (measured: 1 x 8192 x 32768 in 36 us against 21 us for the bytes).  Bytes cost 3.  So x becomes
-// whole numbers: the 128 values of a row's step are scaled by a power of two to |v| <= 2^22 (fp32: 2^30)
-// and split into 3 (4) signed base-256 digits, each a column of the product, whose sums over a group are
-// exact in 32 bits.  A value keeps all bits down to 2^-22 (2^-30) of the largest of its 128, and is off by
-// half of that below: less than the fp32 sums over the groups lose.  A group's sum of (code - 8) times a
-// digit is below 2^22, so it is accumulated on top of the bits of 1.5 2^23 and is a float as it stands;
-// -8 sum(digits) is part of that start.  Infinities and NaN are left out of the digits and added to the
-// sums of their row at the end.
+// whole numbers: the 128 values of a row's step are scaled by a power of two and split into signed base-256
+// digits, each a column of the product, whose sums over a group are exact in 32 bits.  A group's sum of
+// (code - 8) times a digit is below 2^22, so it is accumulated on top of the bits of 1.5 2^23 and is a float
+// as it stands; -8 sum(digits) is part of that start.
 //
-// Measured (device time): 1 x 8192 x 32768 in 25.4 us, 5.4 TB/s of codes and scales, 0.84 of the measured copy
-// rate; 1 x 4096 x 4096 in 5.6 us; 1 x 768 x 768 in 3.5 us, where an empty launch takes 2: bound there by launch, by
-// code that is fetched cold and by the two trips to memory that follow one another.
+// Nothing of x is lost.  What the digits leave of a value far below the largest of its 128 is a float again,
+// and so is all of an infinity or NaN, which has no digits.  Where x is staged these rests are kept by blocks of 32
+// (as many as there is room for, the others are formed again from x) and the row's step is marked; the warp
+// that works on it adds rest times weight in fp32.  The digits are as many as make that rare: 3 a row reach to 2^-23
+// of the largest, so that of normally distributed steps one in 200 (bf16) or 30 (f16) has a rest, 5 of fp32 to
+// 2^-38, one in 100 (4 would leave one in nearly every step), and a single column tile has room for more.  What
+// rests cost (device time): 5 x 8192 x 8192 f16 23.0 us, bf16 21.0; with a value 10^4 times the others in every
+// eighth step 31.3.  What the digits of fp32 cost over 4 that would round x: 2 x 8192 x 8192 18.1 us against 12.9.
+//
+// Measured (device time): 1 x 8192 x 32768 in 24.7 us, 5.6 TB/s of codes and scales, 0.87 of the measured copy
+// rate, but 1 x 8192 x 8192 in 10.1 us, 0.53, where the start of the kernel counts; 1 x 4096 x 4096 in 5.6 us;
+// 1 x 768 x 768 in 3.4 us, where an empty launch takes 2: bound there by launch, by code that is fetched cold and by
+// the two trips to memory that follow one another.
 // ------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void imma16832(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -113,15 +120,16 @@ struct W4Params {
   void* y;
   long long ldx, ldy;
   int* status;
-  int rows, N, K, gated, zeros;
+  int rows, N, K, gated;
   W4Geom g;
   int tiles_q, tiles_r;  // tiles of a CTA, and how many CTAs have one more
-  int chunks, slab_rows;
+  int chunks;
   int tpb;          // row tiles a CTA works on at once (their sums are kept in shared memory)
   int chunk_steps;  // steps of k whose x is in shared memory at once
+  int keep;         // blocks of 32 k whose rests are too
   int align;        // rows of x start on 16-byte boundaries, or 8-byte ones, or others (2)
   int wpr;          // warps that a row of x is staged by
-  uint32_t by_steps, by_rows, by_wpr;  // reciprocals of chunk_steps, the rows of a slab and wpr
+  uint32_t by_steps, by_rows, by_wpr;  // reciprocals of chunk_steps, rows and wpr
 };
 
 // n / d through the reciprocal r = ceil(2^32 / d), for n d < 2^32 (a division costs 100 cycles of a call's 3000)
@@ -135,11 +143,24 @@ constexpr int kDepth = 2;  // copies in flight per warp
 constexpr int kMagicBits = 0x4b400000;  // 1.5 2^23
 constexpr float kMagic = 12582912.f;
 
-template <typename X>
+// |x| < 0.9961 2^(e - 126) is x = 2^(e - 126 - top) (h + 2^-low l) and a rest: h of H digits, at most 0.9961 2^top,
+// which is 127 (1 + 2^8 + ..), l of L, at most 2^(low - 1).  A column tile takes one row of 6 digits (fp32), two of 4
+// (16-bit types); two and more tiles take 5 (3) a row.
+template <typename X, int NT>
 struct Digits {
-  static constexpr int N = sizeof(X) == 4 ? 4 : 3;
-  static constexpr int bits = sizeof(X) == 4 ? 30 : 22;
+  static constexpr int H = sizeof(X) == 2 && NT == 1 ? 4 : 3;
+  static constexpr int L = sizeof(X) == 2 ? 0 : NT == 1 ? 3 : 2;
+  static constexpr int N = H + L;
+  static constexpr int top = H == 4 ? 31 : 23;
+  static constexpr int low = L == 3 ? 23 : L == 2 ? 15 : 0;
+  static constexpr int bits = top + low;
+  static constexpr int rows = 8 * NT / N;  // of x that NT tiles take
 };
+template <typename X>
+constexpr int kPrecision = sizeof(X) == 4 ? 24 : std::is_same<X, __half>::value ? 11 : 8;  // bits that a value has
+constexpr uint32_t kRoundUp = 0x10200;  // added to the bits of a float: to the next power of two from 1.99213 on
+constexpr int kMarkRows = 16;           // a step's marks, one a row: its blocks with a rest, and from bit 4 on their place
+constexpr int kMaxRests = 1024;         // blocks whose rests are kept
 
 // Eight neighbours of a row of x as they are in memory (zeros past its end)
 template <typename X>
@@ -166,17 +187,10 @@ struct Raw8 {
   __device__ __forceinline__ float operator[](int j) const { return to_f32<X>(reinterpret_cast<const X*>(w)[j]); }
 };
 __device__ __forceinline__ bool finite_bits(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
-
-// scale[n, k / g] (code - zero) of the tile's row r at k, from the layout
-template <typename X>
-__device__ float w4_at(const W4Params& p, int t, int r, int k) {
-  const unsigned char* rec = p.data + (static_cast<long long>(t) * p.g.steps + k / 128) * p.g.rec;
-  const int kk = k % 128, b = kk / 32, q = (kk % 32) / 8, j = kk % 8;
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + (r >> 3) * 512 + ((r & 7) * 4 + q) * 16 + b * 4);
-  const int code = (w >> ((j & 3) * 8 + (j >> 2) * 4)) & 15;
-  const int gi = kk / (128 / p.g.gps) * 16 + r;
-  const int zero = p.zeros ? rec[kStepBytes + p.g.gps * 16 * sizeof(X) + gi] & 15 : 8;
-  return to_f32<X>(reinterpret_cast<const X*>(rec + kStepBytes)[gi]) * static_cast<float>(code - zero);
+// What whole numbers of units (a power of two, 1 / unit another) leave of v, exactly; all of it for infinities and NaN
+__device__ __forceinline__ float rest_of(float v, float per_unit, float unit) {
+  const float t = v * per_unit, n = rintf(t);
+  return n == 0.f || !finite_bits(v) ? v : (t - n) * unit;
 }
 
 // NT: tiles of 8 columns (digits of rows).  GPS: groups per step.
@@ -187,9 +201,9 @@ __device__ float w4_at(const W4Params& p, int t, int r, int k) {
 // are taken in their order at the end.
 template <typename X, int NT, int GPS, bool ZERO>
 __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Params p) {
-  constexpr int ND = Digits<X>::N;
+  using D = Digits<X, NT>;
+  constexpr int ND = D::N;
   constexpr int COLS = 8 * NT;
-  constexpr int ROWS = COLS / ND;                             // rows of x a CTA takes
   constexpr int SB = GPS * 16 * static_cast<int>(sizeof(X));  // scale bytes of a step
   constexpr int ZB = ZERO ? GPS * 16 : 0;
   constexpr int kUnit = unit_of(SB + ZB);
@@ -197,21 +211,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
   constexpr int STAGE = kUnit * REC;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint64_t bars[kWarps][kDepth];
-  __shared__ int abort_flag;
-  __shared__ int row_odd[ROWS];  // whether a row has infinities or NaN
+  __shared__ int abort_flag, kept;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row0 = blockIdx.y * ROWS;
-  const int nrow = min(ROWS, p.rows - row0), ncol = nrow * ND;
+  const int nrow = p.rows, ncol = nrow * ND;
   const int pitch = p.chunk_steps * 128 + 16;  // bytes of a column
   unsigned char* ring = smem;
   float* red = reinterpret_cast<float*>(smem + kWarps * kDepth * STAGE);
   // of a group and two neighbouring columns: where their sums start (ZERO: the sums of the digits), their units
   int4* start = reinterpret_cast<int4*>(red + (p.tpb + kWarps - 1) * 16 * COLS);  // [group][COLS / 2]
   unsigned char* xs = reinterpret_cast<unsigned char*>(start + p.chunk_steps * GPS * COLS / 2);  // [column][step][q][b][8]
+  uint16_t* marks = reinterpret_cast<uint16_t*>(xs + ncol * pitch);               // [step][kMarkRows]
+  float* rest_at = reinterpret_cast<float*>(marks + p.chunk_steps * kMarkRows);  // [block][32]
+  bool rests = false;  // whether the chunk has any
   // A thread's first items of x, eight values each, are on their way before the codes: behind those they
   // would wait for as long as the copies in flight take (3 us measured)
   const int sr = div_by(warp, p.by_wpr), si = (warp - sr * p.wpr) * 32 + lane, sn = p.wpr * 32;
-  const X* x = static_cast<const X*>(p.x) + row0 * p.ldx;
+  const X* x = static_cast<const X*>(p.x);
   const X* xr = x + sr * p.ldx;
   const int x_steps = min(p.chunk_steps, p.g.steps);
   auto load_x = [&](Raw8<X>& v, int s0, int ns, int i) {
@@ -220,8 +235,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
   Raw8<X> x0, x1;
   load_x(x0, 0, x_steps, si);
   load_x(x1, 0, x_steps, si + sn);
-  if (tid == 0) abort_flag = 0;
-  if (tid < ROWS) row_odd[tid] = 0;
+  if (tid == 0) abort_flag = kept = 0;
   if (lane == 0) {
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) mbar_init(&bars[warp][d], 1);
@@ -280,47 +294,89 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
       if ((tb == t_lo && ch == 0) || !whole) {
         if (ch > 0 || tb > t_lo) {
           __syncthreads();  // the chunk before is no longer read
+          if (rests) {
+            if (tid == 0) kept = 0;
+            __syncthreads();
+          }
           load_x(x0, s0, ns, si);
           load_x(x1, s0, ns, si + sn);
         }
         const int items = (ns * 16 + 31) / 32 * 32;  // whole warps, since lanes share a step
+        bool any_rest = false;
 #pragma unroll 1
         for (int i = sr < nrow ? si : items; i < items; i += sn) {
-          const Raw8<X> v = x0;
+          const Raw8<X> raw = x0;
           x0 = x1;
           load_x(x1, s0, ns, i + 2 * sn);
+          float v[8], least = INFINITY;
           uint32_t m = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-          const bool odd = __any_sync(0xffffffffu, m >= 0x7f800000u);
-          if (odd) {
-            if (m >= 0x7f800000u) row_odd[sr] = 1;
+          for (int j = 0; j < 8; ++j) {
+            v[j] = raw[j];
+            m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+          }
+          if (__any_sync(0xffffffffu, m >= 0x7f800000u)) {
             m = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (finite_bits(v[j])) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+            for (int j = 0; j < 8; ++j) {
+              v[j] = finite_bits(v[j]) ? v[j] : 0.f;
+              m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+            }
           }
 #pragma unroll
           for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const int e = max(static_cast<int>(m >> 23), 30);  // |x| < 2^(e - 126)
-          const float up = __uint_as_float(static_cast<uint32_t>(Digits<X>::bits + 126 - e + 127) << 23);
-          uint32_t w[8];
+          const int e = max(static_cast<int>((m + kRoundUp) >> 23), D::bits);
+          const float up = __uint_as_float(static_cast<uint32_t>(D::top + 126 - e + 127) << 23);
+          uint32_t w[8], wl[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             // the bytes of (n + B) ^ B are the balanced digits of n (B has 0x80 in every byte but the top one)
-            constexpr uint32_t B = ND == 4 ? 0x808080u : 0x8080u;
-            int n = __float2int_rn(v[j] * up);
-            if (odd && !finite_bits(v[j])) n = 0;
+            constexpr uint32_t B = D::H == 4 ? 0x808080u : 0x8080u, BL = D::L == 3 ? 0x8080u : 0x80u;
+            least = fminf(least, fabsf(v[j]));
+            const float t = v[j] * up;
+            const int n = __float2int_rn(t);
             w[j] = (static_cast<uint32_t>(n) + B) ^ B;
+            if (D::L) wl[j] = (static_cast<uint32_t>(__float2int_rn((t - static_cast<float>(n)) * (1 << D::low))) + BL) ^ BL;
           }
           const int st = i >> 4, b = (i >> 2) & 3, iq = i & 3;
           const bool live = i < ns * 16;
-          int unit = e + 1 - Digits<X>::bits;  // exponent bits of 2^(e - 126 - bits)
+          const int unit0 = e + 1 - D::bits;  // exponent bits of 2^(e - 126 - bits)
+          // all bits of a value from 2^(e - 126 - bits + precision - 1) on are whole units
+          const float whole = __uint_as_float(static_cast<uint32_t>(unit0 + kPrecision<X> - 1) << 23);
+          uint32_t mark = 0;
+          if (__any_sync(0xffffffffu, live && least < whole)) {
+            const float unit = __uint_as_float(static_cast<uint32_t>(unit0) << 23);
+            const float per_unit = __uint_as_float(static_cast<uint32_t>(254 - unit0) << 23);
+            bool rest = false;
 #pragma unroll
-          for (int d = 0; d < ND; ++d) {  // byte d of each
-            const uint32_t sel = 0x0040u + 0x0011u * d;  // bytes d and 4 + d
-            const uint32_t lo = __byte_perm(__byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel), 0x5410);
-            const uint32_t hi = __byte_perm(__byte_perm(w[4], w[5], sel), __byte_perm(w[6], w[7], sel), 0x5410);
+            for (int j = 0; j < 8; ++j) {
+              v[j] = rest_of(raw[j], per_unit, unit);
+              rest |= v[j] != 0.f;
+            }
+            uint32_t with = __ballot_sync(0xffffffffu, rest) >> (lane & 16);  // four lanes a block
+            with |= with >> 2;
+            with = (with | with >> 1) & 0x1111u;
+            with = (with | with >> 3 | with >> 6 | with >> 9) & 15u;
+            int at = 0;  // the order in which rows and steps come here changes where the rests are, and nothing else
+            if (with && (lane & 15) == 0) at = atomicAdd(&kept, __popc(with));
+            at = __shfl_sync(0xffffffffu, at, lane & 16);
+            const bool fits = at + 4 <= p.keep;
+            mark = with | (fits ? at << 4 : 0xfff0);
+            if (fits && (with >> b & 1)) {
+              float* to = rest_at + (at + __popc(with & ((1u << b) - 1))) * 32 + iq * 8;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) to[j] = v[j];
+            }
+            any_rest |= with != 0;
+          }
+          if (live && (lane & 15) == 0) marks[st * kMarkRows + sr] = mark;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            constexpr int L = D::L;
+            const uint32_t(&wd)[8] = d < L ? wl : w;
+            const uint32_t sel = 0x0040u + 0x0011u * (d < L ? d : d - L);  // that byte of each, and 4 bytes on
+            const uint32_t lo = __byte_perm(__byte_perm(wd[0], wd[1], sel), __byte_perm(wd[2], wd[3], sel), 0x5410);
+            const uint32_t hi = __byte_perm(__byte_perm(wd[4], wd[5], sel), __byte_perm(wd[6], wd[7], sel), 0x5410);
             const int col = sr * ND + d;
             if (live) *reinterpret_cast<uint2*>(xs + col * pitch + st * 128 + iq * 32 + b * 8) = make_uint2(lo, hi);
             int sum = __dp4a(static_cast<int>(lo), 0x01010101, __dp4a(static_cast<int>(hi), 0x01010101, 0));
@@ -329,12 +385,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
             if (live && (i & (16 / GPS - 1)) == 0) {
               int* at = reinterpret_cast<int*>(start + (i / (16 / GPS)) * (COLS / 2) + (col >> 1)) + (col & 1);
               at[0] = ZERO ? sum : kMagicBits - 8 * sum;
-              at[2] = unit << 23;
+              at[2] = (unit0 + (d < L ? 8 * d : D::low + 8 * (d - L))) << 23;
             }
-            unit += 8;
           }
         }
-        __syncthreads();
+        rests = __syncthreads_or(any_rest);
       }
 
       int ct = tile_lo, cs = step_lo, cst = 0;
@@ -357,6 +412,62 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
           *d0 = ch == 0 ? make_float2(acc[n][0], acc[n][1]) : make_float2(d0->x + acc[n][0], d0->y + acc[n][1]);
           *d1 = ch == 0 ? make_float2(acc[n][2], acc[n][3]) : make_float2(d1->x + acc[n][2], d1->y + acc[n][3]);
           acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        }
+      };
+      // Adds the rests of row m in step cs, whose record is `rec`: a lane has the codes of eight k of each block
+      auto add_rest = [&](const unsigned char* rec, int m, uint32_t mark) {
+        const int col = m * ND;
+        const float* at = rest_at + (mark >> 4) * 32 + q * 8;
+        const bool in_memory = mark >> 4 != 0xfff;
+        const int k0 = (s0 + cs) * 128 + q * 8;
+        const X* sc = reinterpret_cast<const X*>(rec + kStepBytes) + g;
+        float p0 = 0.f, p1 = 0.f;
+#pragma unroll 1
+        for (uint32_t blocks = mark & 15u; blocks; blocks &= blocks - 1) {
+          const int b = __ffs(blocks) - 1;
+          float r[8];
+          if (in_memory) {
+            const float4 lo = *reinterpret_cast<const float4*>(at), hi = *reinterpret_cast<const float4*>(at + 4);
+            r[0] = lo.x, r[1] = lo.y, r[2] = lo.z, r[3] = lo.w;
+            r[4] = hi.x, r[5] = hi.y, r[6] = hi.z, r[7] = hi.w;
+            at += 32;
+          } else {  // from x again
+            const int4 first = start[cs * GPS * (COLS / 2) + (col >> 1)];
+            const uint32_t unit = static_cast<uint32_t>(col & 1 ? first.w : first.z);
+            Raw8<X> v;
+            v.load(x + m * p.ldx + k0 + b * 32, p.K - k0 - b * 32, p.align);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = rest_of(v[j], __uint_as_float((254u << 23) - unit), __uint_as_float(unit));
+          }
+          uint32_t w0 = *reinterpret_cast<const uint32_t*>(rec + lane * 16 + b * 4);
+          uint32_t w1 = *reinterpret_cast<const uint32_t*>(rec + 512 + lane * 16 + b * 4);
+          const int gi = b * GPS / 4 * 16;
+          const float z0 = 8388608.f + (ZERO ? rec[kStepBytes + SB + gi + g] & 15 : 8);
+          const float z1 = 8388608.f + (ZERO ? rec[kStepBytes + SB + gi + 8 + g] & 15 : 8);
+          float c0 = 0.f, c1 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {  // a code as the low byte of 2^23 is 2^23 + code
+            if (j == 4) w0 >>= 4, w1 >>= 4;
+            const uint32_t sel = 0x7650u + (j & 3);
+            c0 = fmaf(__uint_as_float(__byte_perm(w0 & 0x0f0f0f0fu, 0x4b000000u, sel)) - z0, r[j], c0);
+            c1 = fmaf(__uint_as_float(__byte_perm(w1 & 0x0f0f0f0fu, 0x4b000000u, sel)) - z1, r[j], c1);
+          }
+          p0 = fmaf(to_f32<X>(sc[gi]), c0, p0);
+          p1 = fmaf(to_f32<X>(sc[gi + 8]), c1, p1);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          p0 += __shfl_xor_sync(0xffffffffu, p0, o);
+          p1 += __shfl_xor_sync(0xffffffffu, p1, o);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {  // to the row's first column
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const bool here = n * 8 + 2 * q + h == col;
+            acc[n][h] += here ? p0 : 0.f;
+            acc[n][2 + h] += here ? p1 : 0.f;
+          }
         }
       };
       int f = f_lo;
@@ -435,6 +546,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
 #pragma unroll 2
         for (int u = 0; u < n_steps; ++u) {
           step(u);
+          if (rests) {
+            const uint32_t mark = lane < nrow ? marks[cs * kMarkRows + lane] : 0;
+            for (uint32_t rows = __ballot_sync(0xffffffffu, mark != 0); rows; rows &= rows - 1) {
+              const int m = __ffs(rows) - 1;
+              add_rest(stg + u * REC, m, __shfl_sync(0xffffffffu, mark, m));
+            }
+          }
           ++f;
           if (++cs == ns) {
             flush();
@@ -456,10 +574,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
     __syncthreads();
     // Sums over the warps that had a part of a tile, in their order; then over the digits
     const int log_rows = p.gated ? 3 : 4, orow = 1 << log_rows;
-    for (int i = tid; i < nt * orow * p.slab_rows; i += kWarps * 32) {
+    for (int i = tid; i < nt * orow * nrow; i += kWarps * 32) {
       const int r = i & (orow - 1), tm = i >> log_rows;
-      const int t = div_by(tm, p.by_rows), m = tm - t * p.slab_rows;
-      if (m >= nrow) continue;
+      const int t = div_by(tm, p.by_rows), m = tm - t * nrow;
       const int n = (tb + t) * orow + r;
       if (n >= (p.gated ? p.N / 2 : p.N)) continue;
       float s[2][ND];
@@ -483,16 +600,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
         out[0] += s[0][d];
         out[1] += s[1][d];
       }
-      if (row_odd[m]) {
-        for (int h = 0; h <= p.gated; ++h) {
-          for (int k = 0; k < p.K; ++k) {
-            const float xv = to_f32<X>(x[m * p.ldx + k]);
-            if (!finite_bits(xv)) out[h] += w4_at<X>(p, tb + t, r + 8 * h, k) * xv;
-          }
-        }
-      }
       if (p.gated) out[0] = out[0] / (1.f + expf(-out[0])) * out[1];
-      static_cast<X*>(p.y)[(row0 + m) * p.ldy + n] = from_f32<X>(out[0]);
+      static_cast<X*>(p.y)[m * p.ldy + n] = from_f32<X>(out[0]);
     }
     __syncthreads();
   }
@@ -501,15 +610,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const W4Param
 template <typename X, int NT, int GPS, bool ZERO>
 int launch_stream(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows, int* status,
                   cudaStream_t st) {
-  constexpr int ND = Digits<X>::N;
+  using D = Digits<X, NT>;
+  constexpr int ND = D::N;
   constexpr int COLS = 8 * NT;
-  constexpr int ROWS = COLS / ND;
   constexpr int SIDE = GPS * 16 * static_cast<int>(sizeof(X)) + (ZERO ? GPS * 16 : 0);
   constexpr int kUnit = unit_of(SIDE);
   constexpr int STAGE = kUnit * (kStepBytes + SIDE);
   W4Params p;
   p.data = static_cast<const unsigned char*>(w->data);
-  p.zeros = w->zeros;
   p.x = x;
   p.y = y;
   p.ldx = ldx;
@@ -522,30 +630,30 @@ int launch_stream(const kata_w4_weight* w, const void* x, long long ldx, void* y
   p.g = w4_geom(w);
   const uintptr_t starts = reinterpret_cast<uintptr_t>(x) | (rows > 1 ? static_cast<uintptr_t>(ldx) * sizeof(X) : 0);
   p.align = starts % 16 == 0 ? 16 : starts % 8 == 0 ? 8 : 2;
-  const int ccols = std::min(COLS, rows * ND);
-  const int slabs = (rows + ROWS - 1) / ROWS;
-  const int grid = std::min(p.g.tiles, std::max(1, 148 / slabs));
+  const int ccols = rows * ND;
+  const int grid = std::min(p.g.tiles, 148);
   p.tpb = std::min(NT > 2 ? 4 : 16, (p.g.tiles + grid - 1) / grid);
   const int fixed = kWarps * kDepth * STAGE + (p.tpb + kWarps - 1) * 16 * COLS * 4;
   // x of as many steps as fit, in chunks of one length
-  const int per_step = ccols * 128 + GPS * COLS * 8;
-  const int fit = (kMaxSmem - 2048 - fixed - ccols * 16) / per_step / kUnit * kUnit;
+  const int per_step = ccols * 128 + GPS * COLS * 8 + kMarkRows * 2;
+  const int room = kMaxSmem - 2048 - fixed - ccols * 16;
+  const int fit = (room - 32 * 128) / per_step / kUnit * kUnit;  // beside 32 blocks of rests
   if (fit < kUnit) return KATA_ERR_UNSUPPORTED;
   const int chunks = (p.g.steps + fit - 1) / fit;
   p.tiles_q = p.g.tiles / grid;
   p.tiles_r = p.g.tiles % grid;
-  p.slab_rows = std::min(ROWS, rows);
-  p.wpr = kWarps / p.slab_rows;
-  p.by_rows = recip(p.slab_rows);
+  p.wpr = kWarps / rows;
+  p.by_rows = recip(rows);
   p.by_wpr = recip(p.wpr);
   p.chunk_steps = chunks == 1 ? p.g.steps : ((p.g.steps + chunks - 1) / chunks + kUnit - 1) / kUnit * kUnit;
   p.chunks = (p.g.steps + p.chunk_steps - 1) / p.chunk_steps;
   p.by_steps = recip(p.chunk_steps);
-  const size_t smem = fixed + static_cast<size_t>(p.chunk_steps) * per_step + ccols * 16;
+  p.keep = std::min(kMaxRests, (room - p.chunk_steps * per_step) / 128);
+  const size_t smem = fixed + static_cast<size_t>(p.chunk_steps) * per_step + ccols * 16 + p.keep * 128;
   auto kern = w4_stream_kernel<X, NT, GPS, ZERO>;
   static std::atomic<uint64_t> allowed{0};
   if (int e = allow_smem(reinterpret_cast<const void*>(kern), kMaxSmem - 2048, allowed)) return e;
-  kern<<<dim3(grid, slabs), kWarps * 32, smem, st>>>(p);
+  kern<<<grid, kWarps * 32, smem, st>>>(p);
   return from_cuda(cudaGetLastError());
 }
 
@@ -566,10 +674,9 @@ int launch_groups(const kata_w4_weight* w, const void* x, long long ldx, void* y
 template <typename X>
 int launch_rows(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows,
                 int* status, cudaStream_t st) {
-  const int cols = rows * Digits<X>::N;
-  if (cols <= 8) return launch_groups<X, 1>(w, x, ldx, y, ldy, rows, status, st);
-  if (cols <= 16) return launch_groups<X, 2>(w, x, ldx, y, ldy, rows, status, st);
-  if (cols <= 24) return launch_groups<X, 3>(w, x, ldx, y, ldy, rows, status, st);
+  if (rows <= Digits<X, 1>::rows) return launch_groups<X, 1>(w, x, ldx, y, ldy, rows, status, st);
+  if (rows <= Digits<X, 2>::rows) return launch_groups<X, 2>(w, x, ldx, y, ldy, rows, status, st);
+  if (rows <= Digits<X, 3>::rows) return launch_groups<X, 3>(w, x, ldx, y, ldy, rows, status, st);
   return launch_groups<X, 4>(w, x, ldx, y, ldy, rows, status, st);
 }
 
@@ -1072,15 +1179,15 @@ int w4_check(const kata_w4_weight* w) {
   return KATA_OK;
 }
 
-// Rows that are streamed over.  Up to 16 columns (5 rows, 4 of fp32) the streaming kernel is ahead whatever the
-// size (5 x 8192 x 8192: 20.6 against 23.9 us); up to 32 only while a weight is small and the fixed cost counts
-// (8 x 768 x 768: 5.1 against 9.7 us; 8 x 4096 x 4096: 14.9 against 13.8 us), or where 16-bit rows would have to be
-// laid out for TMA first (7 x 4100 x 5003: 20.2 against 26.6 us).
+// Rows that are streamed over.  Up to two column tiles the streaming kernel is ahead whatever the size (5 x 8192 x 8192:
+// 21.0 against 23.5 us; fp32, 3 rows: 22.4 against 27.6 us); up to four only while a weight is small and the fixed
+// cost counts (8 x 768 x 768: 5.5 against 9.7 us; 8 x 4096 x 4096: 14.9 against 13.8 us; fp32, 6 x 2048 x 2048: 11.3
+// against 13.8 us), or where 16-bit rows would have to be laid out for TMA first (7 x 4100 x 5003: 20.2 against 26.6 us).
 int stream_rows(const kata_w4_weight* w, const void* x, long long ldx) {
   const W4Geom g = w4_geom(w);
   const bool small = static_cast<long long>(g.tiles) * g.steps <= 4096;
-  if (w->dtype == KATA_DTYPE_F32) return small ? 8 : 4;
-  return small || !tma_ready(w->dtype, x, ldx) ? 10 : 5;
+  if (w->dtype == KATA_DTYPE_F32) return small ? Digits<float, 4>::rows : Digits<float, 2>::rows;
+  return small || !tma_ready(w->dtype, x, ldx) ? Digits<__half, 4>::rows : Digits<__half, 2>::rows;
 }
 size_t w4_esize(int dtype) { return dtype == KATA_DTYPE_F32 ? 4 : 2; }
 bool w4_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

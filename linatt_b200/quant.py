@@ -94,8 +94,8 @@ def w4_linear(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
     if rows:
         with _lib.on_device(dev):
             L, xp, ws, n = _lib.lib(), x2.data_ptr(), None, 0
-            # four rows, and 16-bit ones that lie on 16-byte boundaries, never need any
-            if rows > 4 and (w.dtype is torch.float32 or ldx % 8 or xp % 16):
+            # three rows, and 16-bit ones that lie on 16-byte boundaries, never need any
+            if rows > 3 and (w.dtype is torch.float32 or ldx % 8 or xp % 16):
                 n = L.kata_w4_workspace_bytes(w._args, xp, ldx, rows)
                 if n:
                     ws = torch.empty(n, dtype=torch.uint8, device=dev)
