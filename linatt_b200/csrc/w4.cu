@@ -687,8 +687,8 @@ int launch_rows(const kata_w4_weight* w, const void* x, long long ldx, void* y, 
 // unpack warps straight into tensor memory (a row is a TMEM lane, so a thread unpacks words of its own
 // row), and x the B operand by TMA: nothing of A passes through shared memory, whose bandwidth B needs.
 // Codes to floats: a code as a byte beside 0x43 (0x64) is 128 + code in bf16 (1024 + code in f16), and one
-// fused multiply-add leaves unit (code - zero), exactly.  With bf16 the unit is 2^-10: a group's sum stays
-// finite for every finite x; the scale takes it back.  fp32 x is three bf16 parts, each a column.
+// fused multiply-add leaves unit (code - zero), exactly.  With bf16 the unit is 2^-11: a step's sum, of at most
+// 128 times 15 units of x, stays finite for every finite x; the scale takes it back.  fp32 x is three bf16 parts, each a column.
 //
 // A group's products go to one of 2 or 4 accumulators; the drain warps add it, times the rows' scales, to
 // fp32 registers while another one fills, so that scales stay exact.  Unpacking and draining have warps of
@@ -705,13 +705,13 @@ struct Magic;
 template <>
 struct Magic<__nv_bfloat16> {
   static constexpr uint32_t base = 0x43434343u;
-  static constexpr float back = 1024.f;
-  static __device__ __forceinline__ uint32_t offset(uint32_t zero) {  // -(128 + zero) 2^-10
-    const __nv_bfloat162 v = __float2bfloat162_rn(-(128.f + static_cast<float>(zero)) * (1.f / 1024.f));
+  static constexpr float back = 2048.f;
+  static __device__ __forceinline__ uint32_t offset(uint32_t zero) {  // -(128 + zero) 2^-11
+    const __nv_bfloat162 v = __float2bfloat162_rn(-(128.f + static_cast<float>(zero)) * (1.f / 2048.f));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b) {
-    const uint32_t u = 0x3a803a80u;  // 2^-10
+    const uint32_t u = 0x3a003a00u;  // 2^-11
     const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&u),
                                      *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);

@@ -95,6 +95,26 @@ def test_the_smallest_and_the_largest_values(rows, dtype):
     check(w4_linear(full, w), full, W, g, False)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 5, 11, 70])
+def test_the_largest_values_under_the_largest_codes(rows, dtype):
+    """Codes of 15 over zero points of 0, and the reverse: outputs just inside the type's range."""
+    from linatt_b200.quant import W4Weight, w4_linear
+
+    N, K, g = 48, 256, 128
+    code = torch.full((N, K), 15, device="cuda")
+    code[1::2] = 0
+    packed = torch.where(code[:, ::8] == 15, -1, 0).to(torch.int32).contiguous()
+    z = torch.where(code[:, ::g] == 15, 0, 15).to(torch.uint8).contiguous()
+    scales = torch.full((N, 2), 2.0 ** -12, device="cuda", dtype=dtype)
+    W = (code.double() - z.double().repeat_interleave(g, 1)) * 2.0 ** -12
+    w = W4Weight(packed, scales, z, in_features=K, group_size=g)
+    x = torch.full((rows, K), torch.finfo(dtype).max, device="cuda", dtype=dtype)
+    y = w4_linear(x, w)
+    assert torch.isfinite(y).all()
+    check(y, x, W, g, False)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,K,zeros", [(1, 40001, True), (3, 9000, False), (5, 8192, True), (6, 4100, False), (10, 2500, True)])
 def test_more_small_values_than_are_kept_on_chip(rows, K, zeros, dtype):
