@@ -14,7 +14,7 @@
 // q, k and v are rounded once.
 //
 // Measured (device time): 1024 x 6144 bf16 with K = 4, RMS and rotation in 24.4 us, 3.1 TB/s (0.48 of the measured copy
-// rate); 1 x 2304 in 2.2 us, an empty launch.  Bound by latency at 500 threads an SM: with 80 or 64 registers a
+// rate), fp32 without the rotation in 27.4 us; 1 x 2304 in 2.2 us, an empty launch.  Bound by latency at 500 threads an SM: with 80 or 64 registers a
 // thread there are more, but they spill (35 and 53 us).
 #include <algorithm>
 
@@ -144,7 +144,12 @@ __global__ void __launch_bounds__(kQT) qkv_step_kernel(const StepParams p) {
         if (!bad) xin.store(static_cast<T*>(p.ring) + (static_cast<size_t>(b) * S + at) * C + c0);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fdividef(y[i], 1.f + __expf(-y[i]));  // as kata_short_conv_fwd
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(T) == 4)
+          y[i] = y[i] / (1.f + expf(-y[i]));
+        else  // some ten units of fp32 at |a| near 10, far below the 2^-11 and 2^-8 of the outputs
+          y[i] = __fdividef(y[i], 1.f + __expf(-y[i]));
+      }
     }
     if (p.norm_q | p.norm_k) {  // the same for the whole warp, whose heads may be of all three kinds
       float ss = 0.f;

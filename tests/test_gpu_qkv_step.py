@@ -193,3 +193,16 @@ def test_qkv_step_refusals():
         step(x.double(), pos, ring)
     with pytest.raises(RuntimeError):
         step(x.cpu(), pos.cpu(), ring.cpu())
+
+
+def test_silu_of_fp32_channels_to_a_few_units():
+    """a / (1 + exp(-a)) with a given exactly (one tap of weight 1): an exponential of up to 2 units, a sum and a
+    quotient of half a unit each, and a factor below 1 on the first two."""
+    from linatt_b200.qkv_step import QKVStep
+
+    step = QKVStep(num_heads=1, head_k_dim=256, head_v_dim=256, conv_weight=torch.ones(768, 1, device="cuda"))
+    a = torch.linspace(-87, 87, 768 * 64, device="cuda").view(64, 768)
+    q, k, v = step(a, torch.zeros(64, device="cuda", dtype=torch.int64))
+    got = torch.cat((q.flatten(1), k.flatten(1), v.flatten(1)), 1).double()
+    ref = a.double() * torch.sigmoid(a.double())
+    assert ((got - ref).abs() <= 3.01 * 2.0 ** -23 * ref.abs()).all()
