@@ -156,6 +156,8 @@ class KataGenerator:
         """Logits (B, vocab) after one more token (B,) of each sequence."""
         if self.positions is None or token.shape != self.positions.shape:
             raise ValueError("step() follows prefill() of as many sequences")
+        if self.layers[0].cos is not None and self._length >= self.max_positions:
+            raise ValueError(f"the sequences have max_positions={self.max_positions} tokens: none more can be rotated")
         logits = self._step(token)
         self._length += 1
         return logits

@@ -131,3 +131,18 @@ def test_qkv_step_refuses_inputs_on_another_device_than_its_weights(monkeypatch)
     monkeypatch.setattr(torch, "empty", lambda *s, dtype, device: torch.zeros(*s, dtype=dtype))
     with pytest.raises(AssertionError, match="launched"):  # without weights there is nothing to be elsewhere
         free(torch.zeros(2, 24), torch.zeros(2, dtype=torch.int64))
+
+
+def test_generation_refuses_a_step_past_the_rotation_tables():
+    from types import SimpleNamespace
+
+    from linatt_b200.generate import KataGenerator
+
+    gen = KataGenerator.__new__(KataGenerator)
+    gen.layers, gen.positions, gen.max_positions, gen._length = [SimpleNamespace(cos=object())], torch.zeros(2), 5, 4
+    gen._step = lambda token: "stepped"
+    assert gen.step(torch.zeros(2)) == "stepped" and gen._length == 5
+    with pytest.raises(ValueError, match="max_positions"):
+        gen.step(torch.zeros(2))
+    gen.layers[0].cos = None
+    assert gen.step(torch.zeros(2)) == "stepped"

@@ -102,6 +102,26 @@ def test_generate_captured_and_not(head):
     assert torch.equal(greedy[:, 0], gen.prefill(ids).float().argmax(-1))
 
 
+def test_steps_end_at_the_last_position():
+    """The last position that the rotation tables have is used, the next one refused; without a rotation there is none."""
+    from linatt_b200.generate import KataGenerator
+
+    ids = torch.randint(0, 512, (2, 128), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    gen = KataGenerator(make(use_rope=True))
+    gen.prefill(ids[:, :126])
+    for t in (126, 127):
+        assert torch.isfinite(gen.step(ids[:, t])).all()
+    with pytest.raises(ValueError, match="max_positions"):
+        gen.step(ids[:, 0])
+    gen.generate(ids[:, :120], 8)  # the last of eight is drawn and not passed on
+    assert torch.isfinite(gen.step(ids[:, 0])).all()
+    with pytest.raises(ValueError, match="max_positions"):
+        gen.step(ids[:, 0])
+    gen = KataGenerator(make())
+    gen.prefill(ids)
+    assert torch.isfinite(gen.step(ids[:, 0])).all()
+
+
 def test_generate_refusals():
     from linatt_b200.generate import KataGenerator
 
