@@ -624,7 +624,8 @@ KATA_API int kata_qkv_step(const kata_qkv_step_args* args, const void* x, long l
  * ones with exp((x - m) / T) >= min_p; the first token always.  Drawn is the first token in vocabulary
  * order whose inclusive kept mass exceeds u times the whole.  T <= 0: the first token of the order.
  * NaN logits count as -inf, which is never drawn; a row with nothing else gives token -1 and logprob
- * -inf.  logprob is the drawn token's log probability among the kept tokens (0 for T <= 0).
+ * -inf.  logprob is the drawn token's log probability among the kept tokens (0 for T <= 0).  Settings and
+ * numbers that are NaN count as 0.
  * Each setting is a (B) array, or NULL and then the `_all` value.  V <= 2^22.
  * No counterpart in the reference, which does not generate.
  * ------------------------------------------------------------------------------------------- */

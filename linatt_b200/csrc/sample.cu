@@ -799,7 +799,7 @@ struct Sampler {
           mass_parts(d < b_lo ? w : 0.f, h, l);
           sh += h;
           sl += l;
-          const bool k = w >= min_p;
+          const bool k = !(w < min_p);  // as kept()
           kh += k ? h : 0;
           kl += k ? l : 0;
           maybe |= (d >= b_lo && d <= b_hi ? 1u : 0u) << j;
@@ -824,7 +824,7 @@ struct Sampler {
           for (int i = tid; found && i < static_cast<int>(n); i += kST) {
             const u64 o = s.list[i];
             const float w = row.w(key_value(static_cast<uint32_t>(o >> 32)));
-            if (o <= s.cut && w >= min_p) atomicAdd(&s.keep[(static_cast<uint32_t>(o) + skew) / (p.seg / kSW)], mass_of(w));
+            if (o <= s.cut && !(w < min_p)) atomicAdd(&s.keep[(static_cast<uint32_t>(o) + skew) / (p.seg / kSW)], mass_of(w));
           }
           __syncthreads();
         }

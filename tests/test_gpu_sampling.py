@@ -219,6 +219,21 @@ def test_sampling_numbers_at_the_ends():
         assert sample_tokens(logits, u, **par)[0].tolist() == reference(logits, want_u, **par)[0]
 
 
+@pytest.mark.parametrize("V", [3000, 40003])
+def test_sampling_settings_that_are_nan_count_as_zero(V):
+    from linatt_b200.sampling import sample_tokens
+
+    logits, u = draw(5, V, torch.float32, seed=V)
+    logits[4] = logits[4].round()  # thousands of equal logits
+    u[1] = math.nan
+    nan, zero = torch.full((5,), math.nan, device="cuda"), torch.zeros(5, device="cuda")
+    for par in (dict(), dict(top_k=40), dict(top_p=0.9), dict(top_k=2500, top_p=0.9), dict(temperature=0.0)):
+        for name in ("temperature", "top_p", "min_p"):
+            got = sample_tokens(logits, u, **{**par, name: nan})
+            want = sample_tokens(logits, torch.nan_to_num(u, 0.0), **{**par, name: zero})
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (par, name)
+
+
 def test_sampling_does_not_depend_on_the_batch_or_the_layout():
     from linatt_b200.sampling import sample_tokens
 
