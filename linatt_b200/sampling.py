@@ -28,6 +28,8 @@ def _setting(v, name, dtype, B, dev):
         raise ValueError(f"{name} must be a number or a ({B},) tensor, got {tuple(v.shape)}")
     if v.device != dev:
         raise RuntimeError(f"{name} is on {v.device}, the logits on {dev}")
+    if dtype == torch.int32 and v.dtype != dtype:
+        v = v.clamp(0, 1 << 30)  # beyond 32 bits too (the vocabulary is smaller)
     return v.to(dtype).contiguous(), 0
 
 

@@ -146,3 +146,11 @@ def test_generation_refuses_a_step_past_the_rotation_tables():
         gen.step(torch.zeros(2))
     gen.layers[0].cos = None
     assert gen.step(torch.zeros(2)) == "stepped"
+
+
+def test_counts_beyond_32_bits_keep_their_meaning():
+    from linatt_b200.sampling import _setting
+
+    t, _ = _setting(torch.tensor([5, -3, 2 ** 31, 2 ** 32 + 5, 2 ** 62, -2 ** 40]), "top_k", torch.int32, 6, torch.device("cpu"))
+    assert t.dtype == torch.int32 and t[0] == 5
+    assert (t[[1, 5]] <= 0).all() and (t[2:5] >= 2 ** 22).all()  # no more than 2^22 tokens: all of them
