@@ -154,7 +154,7 @@ struct Digits {
   static constexpr int top = H == 4 ? 31 : 23;
   static constexpr int low = L == 3 ? 23 : L == 2 ? 15 : 0;
   static constexpr int bits = top + low;
-  static constexpr int rows = 8 * NT / N;  // of x that NT tiles take
+  static constexpr int rows() { return 8 * NT / N; }  // of x that NT tiles take
 };
 template <typename X>
 constexpr int kPrecision = sizeof(X) == 4 ? 24 : std::is_same<X, __half>::value ? 11 : 8;  // bits that a value has
@@ -674,10 +674,12 @@ int launch_groups(const kata_w4_weight* w, const void* x, long long ldx, void* y
 template <typename X>
 int launch_rows(const kata_w4_weight* w, const void* x, long long ldx, void* y, long long ldy, int rows,
                 int* status, cudaStream_t st) {
-  if (rows <= Digits<X, 1>::rows) return launch_groups<X, 1>(w, x, ldx, y, ldy, rows, status, st);
-  if (rows <= Digits<X, 2>::rows) return launch_groups<X, 2>(w, x, ldx, y, ldy, rows, status, st);
-  if (rows <= Digits<X, 3>::rows) return launch_groups<X, 3>(w, x, ldx, y, ldy, rows, status, st);
-  return launch_groups<X, 4>(w, x, ldx, y, ldy, rows, status, st);
+  if (rows <= Digits<X, 1>::rows()) return launch_groups<X, 1>(w, x, ldx, y, ldy, rows, status, st);
+  if (rows <= Digits<X, 2>::rows()) return launch_groups<X, 2>(w, x, ldx, y, ldy, rows, status, st);
+  if constexpr (sizeof(X) == 4) {
+    if (rows > Digits<X, 3>::rows()) return launch_groups<X, 4>(w, x, ldx, y, ldy, rows, status, st);
+  }
+  return launch_groups<X, 3>(w, x, ldx, y, ldy, rows, status, st);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -785,11 +787,6 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
 __device__ __forceinline__ void arrive_warp(uint64_t* bar) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-               : "memory");
 }
 
 // n MMAs (4 or 2) along k inside one 64-column box of x, one election for all: the MMA warp shares its scheduler
@@ -1009,10 +1006,7 @@ __global__ void __launch_bounds__(GemmSmem<R, sizeof(X) == 4 ? 3 : 1>::threads, 
         uint32_t v[4 * NQ];
 #pragma unroll
         for (int i = 0; i < NQ; ++i) unpack8<T>(b == 0 ? wq[i].x : b == 1 ? wq[i].y : b == 2 ? wq[i].z : wq[i].w, zo[b], v + 4 * i);
-        if constexpr (NQ == 1)
-          tmem_st4(a_at + as * 64 + b * 16, v);
-        else
-          tmem_st8(a_at + as * 64 + b * 16, v);
+        tmem_st8(a_at + as * 64 + b * 16, v);
       }
       if (s % kRun == kRun - 1) arrive_warp(&sm.c_free[s / kRun % kCodeStages]);
       ok = s + 1 >= ns || fetch(s + 1);  // under the stores
@@ -1180,14 +1174,15 @@ int w4_check(const kata_w4_weight* w) {
 }
 
 // Rows that are streamed over.  Up to two column tiles the streaming kernel is ahead whatever the size (5 x 8192 x 8192:
-// 21.0 against 23.5 us; fp32, 3 rows: 22.4 against 27.6 us); up to four only while a weight is small and the fixed
-// cost counts (8 x 768 x 768: 5.5 against 9.7 us; 8 x 4096 x 4096: 14.9 against 13.8 us; fp32, 6 x 2048 x 2048: 11.3
-// against 13.8 us), or where 16-bit rows would have to be laid out for TMA first (7 x 4100 x 5003: 20.2 against 26.6 us).
-int stream_rows(const kata_w4_weight* w, const void* x, long long ldx) {
+// 21.2 against 23.4 us; fp32, 3 rows: 22.7 against 27.4 us; 3 x 4100 x 5003, g 32, zeros: 13.1 against 18.4 us); up to
+// three, four of fp32, only while a weight is small and the fixed cost counts (8 x 768 x 768: 5.5 against 6.5 us; 8 x
+// 2048 x 2048: 7.7 against 11.5, 8 x 4096 x 4096: 14.3 against 11.0 us; fp32, 6 x 2048 x 2048: 11.4 against 13.8, 6 x
+// 8192 x 8192: 50 against 28 us).  Four column tiles of 16-bit rows spill and are behind (10 x 768 x 768: 8.1 against 6.7 us).
+int stream_rows(const kata_w4_weight* w) {
   const W4Geom g = w4_geom(w);
   const bool small = static_cast<long long>(g.tiles) * g.steps <= 4096;
-  if (w->dtype == KATA_DTYPE_F32) return small ? Digits<float, 4>::rows : Digits<float, 2>::rows;
-  return small || !tma_ready(w->dtype, x, ldx) ? Digits<__half, 4>::rows : Digits<__half, 2>::rows;
+  if (w->dtype == KATA_DTYPE_F32) return small ? Digits<float, 4>::rows() : Digits<float, 2>::rows();
+  return small ? Digits<__half, 3>::rows() : Digits<__half, 2>::rows();
 }
 size_t w4_esize(int dtype) { return dtype == KATA_DTYPE_F32 ? 4 : 2; }
 bool w4_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -1224,7 +1219,7 @@ extern "C" int kata_w4_pack(const void* packed, const void* scales, const void* 
 }
 
 extern "C" size_t kata_w4_workspace_bytes(const kata_w4_weight* w, const void* x, long long ldx, long long rows) {
-  if (w4_check(w) || rows <= stream_rows(w, x, ldx) || tma_ready(w->dtype, x, ldx)) return 0;
+  if (w4_check(w) || rows <= stream_rows(w) || tma_ready(w->dtype, x, ldx)) return 0;
   return static_cast<size_t>(rows) * ((w->K + 7) / 8 * 8) * (w->dtype == KATA_DTYPE_F32 ? 6 : 2);
 }
 
@@ -1244,7 +1239,7 @@ extern "C" int kata_w4_linear(const kata_w4_weight* w, const void* x, long long 
   if (need && !w4_al16(workspace)) return KATA_ERR_ALIGN;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int n = static_cast<int>(rows);
-  if (rows <= stream_rows(w, x, ldx)) {
+  if (rows <= stream_rows(w)) {
     if (w->dtype == KATA_DTYPE_BF16) return launch_rows<__nv_bfloat16>(w, x, ldx, y, ldy, n, status, st);
     if (w->dtype == KATA_DTYPE_F16) return launch_rows<__half>(w, x, ldx, y, ldy, n, status, st);
     return launch_rows<float>(w, x, ldx, y, ldy, n, status, st);

@@ -1,7 +1,8 @@
-"""The streaming form of the 4-bit linear layer where a CTA does not have all of x in shared memory at once (long
-rows), where it has more row tiles than it keeps sums of (tall weights), and both.  With 1 to 4 column tiles some 60
-to 150, 30 to 60, 16 to 20 and 12 to 22 steps of 128 k fit, and the sums of 16 row tiles (1 or 2 column tiles) or 4
-are kept: the cases take 2 to 8 chunks, the last one of odd lengths too, and 5, 9 and 17 tiles a CTA."""
+"""The 4-bit linear layer where a CTA of the streaming form does not have all of x in shared memory at once (long
+rows), where it has more row tiles than it keeps sums of (tall weights), and both; and the same beyond its rows.
+With 1 to 4 column tiles some 60 to 150, 30 to 60, 16 to 20 and 20 steps of 128 k fit, and the sums of 16 row tiles
+(1 or 2 column tiles) or 4 are kept: the cases take 2 to 8 chunks, the last one of odd lengths too, and 5 and 17
+tiles a CTA."""
 
 from __future__ import annotations
 
