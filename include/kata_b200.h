@@ -579,7 +579,7 @@ KATA_API size_t kata_w4_bytes(const kata_w4_weight* w);
 KATA_API int kata_w4_pack(const void* packed, const void* scales, const void* zeros, const kata_w4_weight* w,
                           kata_stream_t stream);
 /* y (rows, ldy) = x (rows, ldx) W^T; row strides in elements, both with contiguous columns, of any
- * alignment that their type has.  A few rows are streamed over; more go to the tensor cores, which read x
+ * alignment that their type has, up to 2^21 rows.  A few are streamed over; more go to the tensor cores, which read x
  * by TMA: fp32 rows, and 16-bit rows off 16-byte boundaries, are laid out in the workspace first
  * (kata_w4_workspace_bytes() bytes, 16-byte aligned; 0: none is needed).  status: as for kata_attn_fwd. */
 KATA_API size_t kata_w4_workspace_bytes(const kata_w4_weight* w, const void* x, long long ldx, long long rows);

@@ -14,8 +14,8 @@
 // q, k and v are rounded once.
 //
 // Measured (device time): 1024 x 6144 bf16 with K = 4, RMS and rotation in 24.4 us, 3.1 TB/s (0.48 of the measured copy
-// rate), fp32 without the rotation in 27.4 us; 1 x 2304 in 2.2 us, an empty launch.  Bound by latency at 500 threads an SM: with 80 or 64 registers a
-// thread there are more, but they spill (35 and 53 us).
+// rate), fp32 without the rotation in 27.4 us; 1 x 2304 in 2.2 us, an empty launch.  Bound by latency at 500 threads an
+// SM: with 80 or 64 registers a thread there are more, but they spill (35 and 53 us).
 #include <algorithm>
 
 #include "attn_common.cuh"

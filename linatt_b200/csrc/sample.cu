@@ -23,13 +23,15 @@
 //   found by digits instead: histograms of the distance, then of the bits of the logit and of the index, each within
 //   the bin of the one before.
 //
-// One pass over HBM: a cluster of up to 8 CTAs shares a row (fewer with more rows), each keeping its part
-// in shared memory where it fits (else it is read again, from L2).  Histograms are merged, and lists and sums
+// A cluster of up to 8 CTAs shares a row (fewer with more rows), each keeping its part in shared memory where it
+// fits, so that HBM is read once.  Where it does not (256 x 131072: 192 KB and more a CTA), later passes read it
+// again, from L2 as far as the batch fits there.  Histograms are merged, and lists and sums
 // gathered in the first CTA, through distributed shared memory.  A call of one row is bound by the latency
 // of these steps, a large batch by the instructions of its passes, the exponentials first.
 //
-// Measured (device time): 1 x 32000 top-k and top-p 16 us; 64 x 32000 fp32, temperature only, 14.5 us; 256 x 131072 bf16
-// plain 62 us, top-k 47 us, nucleus 223 us, settings by row 236 us (10.4 us for the bytes).
+// Measured (device time): 1 x 32000 top-k and top-p 16 us; 64 x 32000 fp32, temperature only, 13.5 us; 1 x 131072
+// nucleus 49 us; 256 x 131072 bf16 plain 62 us, top-k 47 us, nucleus 223 us, settings by row 248 us (10.4 us for the
+// bytes), fp32 plain 66 us, nucleus 218 us (20.8 us for the bytes).
 #include <algorithm>
 #include <cmath>
 
@@ -1064,9 +1066,12 @@ using namespace kata;
 
 template <typename T>
 static int launch_sample(SampleParams& p, long long B, cudaStream_t st) {
-  // CTAs a row: up to two an SM, with more than a tile for each warp (1 x 131072 nucleus: 49 us on 8, 228 on one).
+  // CTAs a row: up to two an SM, with more than a tile for each warp (1 x 131072 nucleus: 49 us on 8, 155 on one).
   // Rows of their own settings differ several times in cost, and with one CTA each the last one is waited for: long
-  // ones get twice as many (256 x 131072: 234 against 369 us; with one setting for all, 264 against 223).
+  // ones get twice as many.  From 65536 on that is ahead with every batch (160 rows: 65536 112 against 172 us, 131072
+  // 217 against 306; 75 rows: 65536 80 against 100 us), below it with some (32000: 160 rows 68 against 74 us, but 140
+  // rows 72 against 66; 16384: 290 rows 82 against 69 us).  With one setting for all the rows cost the same, and the
+  // CTAs beyond two an SM wait (256 x 131072 nucleus: 263 against 223 us).
   const bool differ = p.temperature || p.top_k || p.top_p || p.min_p;
   const long long room = differ && p.V >= 65536 ? 592 : 296;
   p.cs = 1;

@@ -97,9 +97,9 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint32_t* __restrict
 // (as many as there is room for, the others are formed again from x) and the row's step is marked; the warp
 // that works on it adds rest times weight in fp32.  The digits are as many as make that rare: 3 a row reach to 2^-23
 // of the largest, so that of normally distributed steps one in 200 (bf16) or 30 (f16) has a rest, 5 of fp32 to
-// 2^-38, one in 100 (4 would leave one in nearly every step), and a single column tile has room for more.  What
-// rests cost (device time): 5 x 8192 x 8192 f16 23.0 us, bf16 21.0; with a value 10^4 times the others in every
-// eighth step 31.3.  What the digits of fp32 cost over 4 that would round x: 2 x 8192 x 8192 18.1 us against 12.9.
+// 2^-38, one in 100 (4 would leave one in two of three), and a single column tile has room for more.  What
+// rests cost (device time): 5 x 8192 x 8192 f16 23.2 us, bf16 21.2; with a value 10^4 times the others in every
+// eighth step 31.3.  What the digits of fp32 cost over 4 that would round x: 2 x 8192 x 8192 18.3 us against 12.9.
 //
 // Measured (device time): 1 x 8192 x 32768 in 24.7 us, 5.6 TB/s of codes and scales, 0.87 of the measured copy
 // rate, but 1 x 8192 x 8192 in 10.1 us, 0.53, where the start of the kernel counts; 1 x 4096 x 4096 in 5.6 us;
@@ -697,8 +697,9 @@ int launch_rows(const kata_w4_weight* w, const void* x, long long ldx, void* y, 
 // their own: in one loop each waits for what the other has just started (1750 cycles a step measured).
 // With few row blocks a cluster's CTAs split k and add their sums through shared memory.
 //
-// Measured (device time): 32 x 8192 x 8192 in 24.5 us, 64 x 4096 x 16384 gated in 31.9 us, 512 x 4096 x 4096 in
-// 34.4 us (500 TFLOP/s).  Bound by issue: the unpack warps' 11 instructions a word, and the MMA warp, which takes
+// Measured (device time): 8 to 32 x 8192 x 8192 in 23.8 us, 8 x 8192 x 32768 in 74.9 us (two rounds of 256 row blocks on
+// 148 SMs), 64 x 4096 x 16384 gated in 27.5 us, 512 x 4096 x 4096 in 34.4 us (500 TFLOP/s) and 2048 in 130 us; fp32
+// 64 x 4096 x 4096 in 18.4 us, 512 in 74.4 us.  Bound by issue: the unpack warps' 11 instructions a word, and the MMA warp, which takes
 // 750 cycles for a step's 8 MMAs beside them, whatever their width.
 // ------------------------------------------------------------------------------------------------
 

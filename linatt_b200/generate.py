@@ -174,7 +174,8 @@ class KataGenerator:
                  use_graph: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
         """(tokens, logprobs), each (B, max_new_tokens), after the prompts input_ids (B, T).  ``u``
         (max_new_tokens, B) fp32: the uniform numbers of the draws (default: from ``generator``); the other
-        settings as :func:`sample_tokens`."""
+        settings as :func:`sample_tokens`.  The prompts are of one length, and every sequence gets all new tokens (no
+        token ends one).  From four new tokens on, every call captures its step anew."""
         B, T = input_ids.shape
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be at least 1")

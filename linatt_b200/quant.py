@@ -74,7 +74,7 @@ class W4Weight:
 
 def w4_linear(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
     """y = x W^T of x (..., in_features) in the weight's dtype, or silu(gate) * up for a gated weight:
-    (..., out_features).  Products are exact and summed in fp32; y is rounded once.  Any number of rows."""
+    (..., out_features).  Products are exact and summed in fp32; y is rounded once.  Up to 2^21 rows."""
     if x.device != w.device:
         _lib.require_cuda(x)
         raise RuntimeError(f"x is on {x.device}, the weight on {w.device}")
