@@ -561,7 +561,8 @@ KATA_API int kata_add_rmsnorm_bwd(const kata_add_rmsnorm_args* args, kata_stream
  * and, for a gated weight (gate rows 0..N/2-1, up rows N/2..N-1), y = silu(gate) * up with N/2 columns.
  * The codes and scales are exact in the products, which are summed in fp32 per group; only y is rounded.
  * `data` is in this library's tile layout, written once by kata_w4_pack into kata_w4_bytes() bytes, 16-byte
- * aligned.  group: 32, 64 or a multiple of 128.  dtype is that of x, y and the scales (fp32 x is used in full).
+ * aligned.  group: 32, 64 or a multiple of 128.  dtype is that of x, y and the scales (fp32 x is used in full; where
+ * rows go to the tensor cores, down to bits of 2^-133).
  * No counterpart in the reference, whose layers keep 16- or 32-bit weights.
  * ------------------------------------------------------------------------------------------- */
 typedef struct {

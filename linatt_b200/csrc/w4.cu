@@ -740,8 +740,8 @@ __device__ __forceinline__ void unpack8(uint32_t word, uint32_t offset, uint32_t
   out[3] = Magic<T>::fma2(__byte_perm(hi, Magic<T>::base, 0x4342), offset);
 }
 
-// An fp32 value as three bf16 parts, each the leading 8 bits of what is left: exact together, and no
-// part overflows.  Infinities and NaN stay in the first part.
+// An fp32 value as three bf16 parts, each the leading 8 bits of what is left: exact together (but for bits below
+// 2^-133, which bf16 does not have: of values from 2^-110 on nothing), and no part overflows.  Infinities and NaN stay in the first part.
 __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
   const float a = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
   const bool fin = finite_bits(x);
